@@ -248,6 +248,51 @@ int mta_fused_fwd_host(const void* q, const void* k, const void* v, const void* 
 int mta_host_pipeline_release(void);
 
 /*
+ * Token by token over a paged cache (these entry points have no counterpart in the reference, which recomputes the whole prefix).
+ * A cache of one layer, all in device memory:
+ *   k_pages, v_pages  (pages, kv_heads, page, D): `page` tokens of every head; a power of two from 16 on
+ *   q_hist            (slots, ring, H, D): the last queries of every sequence, position p at p % ring
+ *   table             (slots, table_width): the page numbers of every sequence, in order
+ *   lengths           (slots): tokens of every sequence, the newest among them
+ * slot_ids (B) says which slot each batch row is; NULL: row b is slot b.  H is a multiple of kv_heads: query head h reads key-value
+ * head h / (H / kv_heads).  D is a multiple of 8, at most 256 (float32: 128).  All pointers to queries, keys and values and the
+ * workspace are 16-byte aligned.  A slot, page, length or count that is out of range is neither read nor written: such a sequence counts
+ * as empty, such a page as zeros, and mta_cache_status() reports it.
+ *
+ * mta_cache_append writes new tokens: k, v (B,kv_heads,T,D) and q (B,H,T,D), `strides` the nine strides in elements of k's, v's and
+ * q's batch rows, heads and tokens (multiples of 16 bytes; elements of a row are contiguous).  Row b has counts[b] <= T tokens (NULL: T),
+ * which become the last of lengths[slot]; of its queries the last `ring` are kept.  No slot may stand in the batch twice.
+ *
+ * mta_cache_copy copies page src[i] to page dst[i] (n pairs, keys and values) and the queries of slot slot_src[i] to slot_dst[i]
+ * (n_slots pairs), in each of `layers` pools that lie one behind another.  No destination may be named twice or be a source.
+ *
+ * mta_decode_fwd is the MTA module (mta_fused_fwd) for the newest token of every row: o (B,H,D).  The last cq + cq2 - 1 <= ring
+ * queries are read (at most 32); kernels have at most 33 key taps, odd or even, centred as mta_conv2d_fwd centres them; H <= 128.
+ * mta_conv_attn_decode_fwd is the conv attention (mta_conv_attn_fwd, causal) likewise; it reads the last cq queries.
+ * Both: an empty sequence gets zeros; no length exceeds max_length (which sizes the workspace and the split of the work: inside a
+ * captured graph pass the longest that the graph is to serve); at most 1024 rows.  Sums, softmax statistics, scores and weights are float32;
+ * the result is rounded once, so it is nearer to exact than the whole-sequence forward, which rounds between stages.
+ */
+int mta_cache_append(const void* k, const void* v, const void* q, const long long* strides, const int* counts, void* k_pages, void* v_pages,
+                     void* q_hist, const int* table, const int* lengths, const int* slot_ids, int B, int T, int slots, int table_width,
+                     int pages, int page, int ring, int H, int kv_heads, int D, int dtype, void* stream);
+int mta_cache_copy(void* k_pages, void* v_pages, const int* src, const int* dst, int n, long long page_bytes, int pages, void* q_hist,
+                   const int* slot_src, const int* slot_dst, int n_slots, long long slot_bytes, int slots, int layers, void* stream);
+size_t mta_decode_workspace_bytes(int B, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2, int max_length);
+int mta_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const int* slot_ids,
+                   const void* w1, const void* W1, const void* w2, const void* W2, void* o, void* workspace, size_t workspace_bytes, int B,
+                   int slots, int table_width, int pages, int page, int ring, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2,
+                   int max_length, int dtype, int w_dtype, void* stream);
+size_t mta_conv_attn_decode_workspace_bytes(int B, int H, int kv_heads, int D, int cq, int ck, int max_length);
+int mta_conv_attn_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages, const int* table, const int* lengths,
+                             const int* slot_ids, const void* w, void* o, void* workspace, size_t workspace_bytes, int B, int slots,
+                             int table_width, int pages, int page, int ring, int H, int kv_heads, int D, int cq, int ck, int max_length,
+                             float scale, int dtype, int w_dtype, void* stream);
+/* Synchronises `stream` and reports whether a cache call on this device since the last check met something out of range (returns 1 and
+ * clears the condition). */
+int mta_cache_status(void* stream);
+
+/*
  * Stage tracing of mta_fused_fwd (calling thread): after mta_set_stage_trace(1) every forward records a CUDA event
  * on its stream before each stage and after the last.  mta_stage_times_ms waits for the latest forward and writes
  * the device time of each of its stages (milliseconds) and, if `names` is not NULL, a static name per stage;

@@ -66,6 +66,13 @@ SIGNATURES = {
     "mta_fused_fwd_dropout": (_i, [_vp] * 9 + [_sz] + [_i] * 13 + [_f, ctypes.c_ulonglong, _vp]),
     "mta_fused_fwd_host": (_i, [_vp] * 8 + [_i] * 12),
     "mta_host_pipeline_release": (_i, []),
+    "mta_cache_append": (_i, [_vp] * 11 + [_i] * 11 + [_vp]),
+    "mta_cache_copy": (_i, [_vp] * 4 + [_i, ctypes.c_longlong, _i] + [_vp] * 3 + [_i, ctypes.c_longlong, _i, _i, _vp]),
+    "mta_decode_workspace_bytes": (_sz, [_i] * 9),
+    "mta_decode_fwd": (_i, [_vp] * 12 + [_sz] + [_i] * 16 + [_vp]),
+    "mta_conv_attn_decode_workspace_bytes": (_sz, [_i] * 7),
+    "mta_conv_attn_decode_fwd": (_i, [_vp] * 9 + [_sz] + [_i] * 12 + [_f, _i, _i, _vp]),
+    "mta_cache_status": (_i, [_vp]),
     "mta_set_stage_trace": (_i, [_i]),
     "mta_stage_times_ms": (_i, [_vp, _vp, _i]),
 }
@@ -139,6 +146,13 @@ def device_status(device=None) -> None:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     with torch.cuda.device(dev):
         check(lib().mta_device_status(stream_ptr(dev)), "mta_device_status")
+
+
+def cache_status(device=None) -> None:
+    """Synchronises the current stream and raises if a cache call met a page, slot, length or count out of range."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        check(lib().mta_cache_status(stream_ptr(dev)), "mta_cache_status")
 
 
 def set_variant(key: str, value: int) -> None:

@@ -1,0 +1,243 @@
+// What the kernels over a paged cache share: the cache's description, the bounds checks of what it says, and the tiles of 16 keys
+// and values that a warp holds in registers.
+#pragma once
+
+#include "kernels.cuh"
+#include "tc05.cuh"
+
+namespace mta {
+
+// A paged cache of one layer.  k, v: (pages, kv_heads, page, D); q_hist: (slots, ring, H, D), the query of position p at p % ring;
+// table: (slots, table_width) page numbers; lengths: (slots) tokens, the newest among them.  Batch row b is slot slot_ids[b] (b when
+// null).  `page` is a power of two from 16 on, so that 16 keys from a multiple of 16 on lie in one page.
+struct PagedCache {
+    const void* q_hist;
+    const void* k;
+    const void* v;
+    const int* table;
+    const int* lengths;
+    const int* slot_ids;
+    int slots, table_width, pages, page_shift, ring, H, kv_heads, D;
+    int max_length;      // no sequence of the call is longer
+    int* err;            // the device's flags: [1] is raised by what a table, length or slot says wrongly
+
+    // Raises the flag of a bad table, length or slot: that part of the cache is not touched, mta_cache_status() reports it.
+    __device__ void bad() const { atomicExch(err + 1, 1); }
+    __device__ int slot(int b) const { return slot_ids ? __ldg(slot_ids + b) : b; }
+    // Tokens of batch row b; 0 where slot or length are out of range.
+    __device__ int length(int b) const {
+        const int s = slot(b);
+        if ((unsigned)s >= (unsigned)slots) { bad(); return 0; }
+        const int n = __ldg(lengths + s);
+        if (n < 0 || n > max_length) { bad(); return 0; }
+        return n;
+    }
+    // Element offset of (kv head, token) in the pools for a slot in range; -1 where the table names no page.
+    __device__ long at(int s, int kv_head, int token) const {
+        const int p = __ldg(table + (long)s * table_width + (token >> page_shift));
+        if ((unsigned)p >= (unsigned)pages) { bad(); return -1; }
+        return ((((long)p * kv_heads + kv_head) << page_shift) + (token & ((1 << page_shift) - 1))) * D;
+    }
+};
+
+constexpr int KEYS = 16;                 // keys of a tile: the rows of one mma.sync
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 keys of one head in a warp's registers, DMAX >= D elements each.  Lane (g, t) = (lane / 4, lane % 4) holds of rows g and g + 8
+// the 16 bytes at chunk c * 64 + t * 16: whole 16-byte loads, four lanes on 64 contiguous bytes.  An mma sums over its k index in
+// any order, so the elements of a lane's 16 bytes may stand for any k as long as the queries are read the same way.
+template <typename T, int DMAX> struct KeyTile {
+    static constexpr int CH = DMAX * (int)sizeof(T) / 64;
+    static constexpr int EPL = 16 / (int)sizeof(T);      // elements in 16 bytes
+    uint4 r[2][CH];
+
+    // Rows base, base + 1, ... of which `live` exist; the others are zero and not read.  base < 0: none exists.
+    __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const bool on = base >= 0 && g + 8 * x < live;
+            const T* row = pool + (on ? base + (long)(g + 8 * x) * D : 0);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int e = (c * 4 + t) * EPL;
+                r[x][c] = on && e < D ? __ldg(reinterpret_cast<const uint4*>(row + e)) : make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+
+    // Scores of the 16 keys with NT * 8 query rows: acc[n][0..1] = key g, rows 8n + 2t, 8n + 2t + 1; acc[n][2..3] = key g + 8.
+    // q(row, c) gives this lane's 16 bytes (chunk c, position t) of a query row.
+    template <int NT, typename Q> __device__ __forceinline__ void score(float (&acc)[NT][4], int lane, Q q) const {
+        if constexpr (sizeof(T) == 2) {
+            const int g = lane >> 2;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const uint4 b = q(8 * n + g, c);
+                    mma_16816<T>(acc[n], r[0][c].x, r[1][c].x, r[0][c].y, r[1][c].y, b.x, b.y);
+                    mma_16816<T>(acc[n], r[0][c].z, r[1][c].z, r[0][c].w, r[1][c].w, b.z, b.w);
+                }
+            }
+        } else {
+            // float32 on FMAs: each lane sums its quarter of the elements for eight rows, then the four lanes of a key exchange
+            // halves twice, which leaves every lane with the two rows that the mma layout gives it
+            const int t = lane & 3;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float p[2][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[0][j] = p[1][j] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 b = q(8 * n + j, c);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            p[x][j] = fmaf(__uint_as_float(r[x][c].x), __uint_as_float(b.x), p[x][j]);
+                            p[x][j] = fmaf(__uint_as_float(r[x][c].y), __uint_as_float(b.y), p[x][j]);
+                            p[x][j] = fmaf(__uint_as_float(r[x][c].z), __uint_as_float(b.z), p[x][j]);
+                            p[x][j] = fmaf(__uint_as_float(r[x][c].w), __uint_as_float(b.w), p[x][j]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float h[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float give = t & 2 ? p[x][j] : p[x][j + 4], keep = t & 2 ? p[x][j + 4] : p[x][j];
+                        h[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float give = t & 1 ? h[j] : h[j + 2], keep = t & 1 ? h[j + 2] : h[j];
+                        acc[n][2 * x + j] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// The elements of 16 bytes as floats.
+template <typename T> __device__ __forceinline__ void unpack16(uint4 u, float (&f)[16 / sizeof(T)]);
+template <> __device__ __forceinline__ void unpack16<float>(uint4 u, float (&f)[4]) {
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+template <> __device__ __forceinline__ void unpack16<__nv_bfloat16>(uint4 u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void unpack16<__half>(uint4 u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = p.x; f[2 * i + 1] = p.y;
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack16(const float* f);
+template <> __device__ __forceinline__ uint4 pack16<float>(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <> __device__ __forceinline__ uint4 pack16<__nv_bfloat16>(const float* f) {
+    return make_uint4(pack2<__nv_bfloat16>(f[0], f[1]), pack2<__nv_bfloat16>(f[2], f[3]), pack2<__nv_bfloat16>(f[4], f[5]), pack2<__nv_bfloat16>(f[6], f[7]));
+}
+template <> __device__ __forceinline__ uint4 pack16<__half>(const float* f) {
+    return make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]), pack2<__half>(f[4], f[5]), pack2<__half>(f[6], f[7]));
+}
+
+// 16 values of one head in a warp's registers: ROWLANES lanes side by side hold a row, the warp SUBS rows at a time.  The product
+// with the weights stays on float32 FMAs: it has one row of weights per head, a sixteenth of what an mma computes, and the weights
+// would have to be rounded.
+template <typename T, int DMAX> struct ValueTile {
+    static constexpr int EPL = 16 / (int)sizeof(T);
+    static constexpr int ROWLANES = DMAX / EPL;
+    static constexpr int SUBS = 32 / ROWLANES;
+    static constexpr int STEPS = KEYS / SUBS;
+    uint4 r[STEPS];
+
+    __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
+        const int sub = lane / ROWLANES, e = (lane % ROWLANES) * EPL;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const bool on = base >= 0 && i * SUBS + sub < live && e < D;
+            r[i] = on ? __ldg(reinterpret_cast<const uint4*>(pool + base + (long)(i * SUBS + sub) * D + e)) : make_uint4(0, 0, 0, 0);
+        }
+    }
+};
+
+// Work on sequences of different lengths is cut into `workers` equal runs of tiles; a run may begin in one sequence (line) and end
+// in another.  Tile range of worker w of n tiles, and the worker that has tile x.
+__device__ __forceinline__ long run_begin(long w, long n, long workers) { return w * n / workers; }
+__device__ __forceinline__ long run_owner(long x, long n, long workers) { return ((x + 1) * workers - 1) / n; }
+
+// before[b] = tiles of `1 << shift` keys in sequences 0..b-1, for b up to and with B; by the first warp of the block.
+__device__ __forceinline__ void count_tiles(const PagedCache& c, int B, int shift, int* before, int* lens) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int sum = 0;
+        for (int b0 = 0; b0 < B; b0 += 32) {
+            const int len = b0 + lane < B ? c.length(b0 + lane) : 0;
+            int n = (len + (1 << shift) - 1) >> shift;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += up;
+            }
+            if (b0 + lane < B) {
+                before[b0 + lane + 1] = sum + n;
+                lens[b0 + lane] = len;
+            }
+            sum += __shfl_sync(0xffffffffu, n, 31);
+        }
+        if (lane == 0) before[0] = 0;
+    }
+}
+
+// The last index b with before[b] <= x, x < before[B].
+__device__ __forceinline__ int find_line(const int* before, int B, long x) {
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// SMs of a B200.  The cuts of the work follow from the call's sizes alone, so that a workspace's size can be asked for without a device.
+constexpr int DECODE_SMS = 148;
+constexpr int DECODE_MAX_BATCH = 1024;   // batch rows of one call: their tile counts stand in shared memory
+constexpr int DECODE_MAX_TAPS = 33;      // key taps: a tile's neighbours hold what its conv reaches
+constexpr int DECODE_MAX_ROWS = 32;      // query rows that one new token looks at
+
+// Launchers (paged_cache.cu, paged_conv_attn.cu, paged_mta.cu); abi_paged.cu has checked their arguments.  strides: elements between
+// batch rows, heads and tokens of k, v and q.
+int cache_append_launch(const PagedCache& cache, const void* k, const void* v, const void* q, const long* strides, const int* counts, int B, int T,
+                        int dtype, cudaStream_t st);
+int cache_copy_launch(void* k_pages, void* v_pages, const int* src, const int* dst, int n, long page_bytes, int pages, void* q_hist, const int* slot_src,
+                      const int* slot_dst, int n_slots, long slot_bytes, int slots, int layers, cudaStream_t st);
+size_t conv_attn_decode_workspace(int B, int H, int kv_heads, int D, int cq, int max_length);
+int conv_attn_decode_launch(const PagedCache& cache, const void* w, int w_dtype, void* out, void* workspace, int B, int cq, int ck, float scale, int dtype,
+                            cudaStream_t st);
+// Fails where the heads' scores or probabilities do not fit in shared memory.
+int mta_decode_workspace(int B, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2, int max_length, size_t* bytes);
+int mta_decode_launch(const PagedCache& cache, const void* w1, const void* W1, const void* w2, const void* W2, int w_dtype, void* out, void* workspace, int B,
+                      int cq, int ck, int cq2, int ck2, int dtype, cudaStream_t st);
+
+}  // namespace mta
