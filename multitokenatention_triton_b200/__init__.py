@@ -7,8 +7,9 @@ from .convolution_2d import Conv2dTriton, Conv2dTritonFunction
 from .linear_head import TritonLinearHead, TritonLinearHeadFunction
 from .conv_attention import TritonAttention, TritonConvAttention
 from .mta_attention import MTAAttentionTriton
+from .paged_cache import CacheBatch, CacheFullError, PagedKVCache
 
 __all__ = [
     "Conv2dTriton", "Conv2dTritonFunction", "TritonLinearHead", "TritonLinearHeadFunction",
-    "TritonAttention", "TritonConvAttention", "MTAAttentionTriton",
+    "TritonAttention", "TritonConvAttention", "MTAAttentionTriton", "PagedKVCache", "CacheBatch", "CacheFullError",
 ]

@@ -36,3 +36,25 @@ class TritonConvAttention(nn.Module):
 
     def forward(self, Q, K, V, causal, softmax_scale):
         return TritonAttention.apply(Q, K, V, self.weight, causal, softmax_scale), None
+
+    @property
+    def query_history(self) -> int:
+        """Queries that a cache has to keep for this module."""
+        return self.kernel_size[0]
+
+    def forward_cached(self, Q, K, V, cache, batch, softmax_scale=None, layer: int = 0, max_length=None):
+        """forward (causal) for new tokens of the sequences of a PagedKVCache: Q (B,H,T,D), K, V (B,kv heads,T,D) -> ((B,H,T,D), None), and the tokens
+        are kept.  T, `batch` and `max_length` as in MTAAttentionTriton.forward_cached."""
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, K, V, self.weight)):
+            raise NotImplementedError("TritonConvAttention with a cache has no backward pass: call it under torch.no_grad()")
+        prompt = Q.size(2) != 1
+        if prompt and not batch.from_empty:
+            raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
+        cache.append(batch, K, V, Q, layer)
+        if prompt:
+            group = Q.size(1) // K.size(1)
+            if group > 1:
+                K, V = K.repeat_interleave(group, dim=1), V.repeat_interleave(group, dim=1)
+            return ops.conv_attn_fwd(Q, K, V, self.weight, True, softmax_scale), None
+        return ops.conv_attn_decode_fwd(*cache.layer(layer), self.weight, softmax_scale, batch.max_length if max_length is None else max_length,
+                                        slots=batch.slot_ids), None

@@ -11,6 +11,8 @@ seven steps one by one through the stand-alone entry points, which keeps every 1
 the reference.  `use_mask=True` takes the reference's explicit masks (None, boolean, additive, padding or (1,1,S,S)): None
 and a boolean (batch, keys) mask without a gradient or dropout run as the fused causal forward, the second through
 mta_masked_fwd; the others run stage by stage over full score planes.
+
+`forward_cached` generates token by token over a PagedKVCache (paged_cache.py), which the reference has no counterpart of.
 """
 import torch
 import torch.nn as nn
@@ -63,16 +65,16 @@ class MTAAttentionTriton(nn.Module):
         if not self.causal:
             raise NotImplementedError("MTAAttentionTriton without a mask requires causal=True, as in the reference's benchmarks")
         dropping = self.training and self.dropout > 0.0
-        if self.fused and not (torch.is_grad_enabled() and any(t.requires_grad for t in (xq, xk, xv, *self.parameters()))):
+        w1, w2 = self.mta_conv_triton.effective_weight(), self.mta_conv_after_sm_triton.effective_weight()
+        odd = w1.size(-1) % 2 and w2.size(-1) % 2
+        if self.fused and odd and not (torch.is_grad_enabled() and any(t.requires_grad for t in (xq, xk, xv, *self.parameters()))):
             # F.dropout(scores, p=self.dropout, training=self.training) (mta_attention_triton.py:87) runs inside the last
             # kernel; its seed is drawn from torch's CPU generator, so torch.manual_seed makes a forward repeatable
             seed = int(torch.randint(0, 2 ** 62, (1,), dtype=torch.int64).item()) if dropping else 0
-            out = ops.mta_fused_fwd(xq, xk, xv, self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
-                                    self.mta_conv_after_sm_triton.effective_weight(), self.wposm_triton.weight, causal=True,
+            out = ops.mta_fused_fwd(xq, xk, xv, w1, self.wpsm_triton.weight, w2, self.wposm_triton.weight, causal=True,
                                     dropout_p=self.dropout if dropping else 0.0, dropout_seed=seed)
             return out.transpose(1, 2)
-        w1, w2 = self.mta_conv_triton.effective_weight(), self.mta_conv_after_sm_triton.effective_weight()
-        if self.fused and not dropping and xk.shape == xq.shape and xv.shape == xq.shape and w1.size(-1) % 2 and w2.size(-1) % 2:
+        if self.fused and odd and not dropping and xk.shape == xq.shape and xv.shape == xq.shape:
             return MTAFunction.apply(xq, xk, xv, w1, self.wpsm_triton.weight, w2, self.wposm_triton.weight).transpose(1, 2)
         # Stage by stage: `fused=False`, a gradient with dropout, cross attention, even key extents.  Every stage is differentiable,
         # the conv and the head mix through their backward kernels, the scores, the softmax and the product with V through autograd_ops.
@@ -164,6 +166,36 @@ class MTAAttentionTriton(nn.Module):
                                    causal=True, out=out,
                                    chunk_batch=chunk_batch)
         return o.transpose(1, 2)
+
+    @property
+    def query_history(self) -> int:
+        """Queries that a cache has to keep for this module: the newest and those that the two convs reach back to."""
+        return self.mta_conv_triton.weight.size(1) + self.mta_conv_after_sm_triton.weight.size(1) - 1
+
+    def forward_cached(self, xq, xk, xv, cache, batch, layer: int = 0, max_length=None):
+        """forward for new tokens of the sequences of a PagedKVCache: xq (B,H,T,D), xk, xv (B,kv heads,T,D) -> (B,T,H,D), and the tokens are kept.
+        `batch` is what cache.extend() gave.  One token per sequence (T = 1) attends to all of its sequence; several are a
+        prompt: the sequences were empty before, tokens behind a row's count are padding, and so are their outputs.  `max_length` (T = 1):
+        the longest sequence that the call is to serve, where it is captured into a graph and replayed for longer ones."""
+        if not self.causal:
+            raise NotImplementedError("MTAAttentionTriton with a cache requires causal=True")
+        if self.training and self.dropout > 0.0:
+            raise NotImplementedError("MTAAttentionTriton with a cache has no dropout: switch to eval()")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (xq, xk, xv, *self.parameters())):
+            raise NotImplementedError("MTAAttentionTriton with a cache has no backward pass: call it under torch.no_grad()")
+        prompt = xq.size(2) != 1
+        if prompt and not batch.from_empty:
+            raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
+        cache.append(batch, xk, xv, xq, layer)
+        if prompt:
+            group = xq.size(1) // xk.size(1)
+            if group > 1:
+                xk, xv = xk.repeat_interleave(group, dim=1), xv.repeat_interleave(group, dim=1)
+            return self.forward(xq, xk, xv, None, None)
+        out = ops.mta_decode_fwd(*cache.layer(layer), self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
+                                 self.mta_conv_after_sm_triton.effective_weight(), self.wposm_triton.weight,
+                                 batch.max_length if max_length is None else max_length, slots=batch.slot_ids)
+        return out.transpose(1, 2)
 
     def reset_mta_parameters(self, init_std=None):
         """Initialise as the reference does (mta_attention_triton.py:129-145): conv kernels by
