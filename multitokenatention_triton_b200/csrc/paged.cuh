@@ -77,16 +77,15 @@ template <typename T, int DMAX> struct KeyTile {
     }
 
     // Scores of the 16 keys with NT * 8 query rows: acc[n][0..1] = key g, rows 8n + 2t, 8n + 2t + 1; acc[n][2..3] = key g + 8.
-    // q(row, c) gives this lane's 16 bytes (chunk c, position t) of a query row.
+    // 16 bits: q(n, c) gives 16 bytes (chunk c, position t) of this lane's own query row 8n + g; float32: q(row, c) of any row.
     template <int NT, typename Q> __device__ __forceinline__ void score(float (&acc)[NT][4], int lane, Q q) const {
         if constexpr (sizeof(T) == 2) {
-            const int g = lane >> 2;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const uint4 b = q(8 * n + g, c);
+                    const uint4 b = q(n, c);
                     mma_16816<T>(acc[n], r[0][c].x, r[1][c].x, r[0][c].y, r[1][c].y, b.x, b.y);
                     mma_16816<T>(acc[n], r[0][c].z, r[1][c].z, r[0][c].w, r[1][c].w, b.z, b.w);
                 }
@@ -97,9 +96,9 @@ template <typename T, int DMAX> struct KeyTile {
             const int t = lane & 3;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float p[2][8];
+                float2 p[2][8];                              // sums of even and odd elements
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[0][j] = p[1][j] = 0.0f;
+                for (int j = 0; j < 8; ++j) p[0][j] = p[1][j] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -107,19 +106,21 @@ template <typename T, int DMAX> struct KeyTile {
                         const uint4 b = q(8 * n + j, c);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            p[x][j] = fmaf(__uint_as_float(r[x][c].x), __uint_as_float(b.x), p[x][j]);
-                            p[x][j] = fmaf(__uint_as_float(r[x][c].y), __uint_as_float(b.y), p[x][j]);
-                            p[x][j] = fmaf(__uint_as_float(r[x][c].z), __uint_as_float(b.z), p[x][j]);
-                            p[x][j] = fmaf(__uint_as_float(r[x][c].w), __uint_as_float(b.w), p[x][j]);
+                            p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].x), __uint_as_float(r[x][c].y)),
+                                                 make_float2(__uint_as_float(b.x), __uint_as_float(b.y)), p[x][j]);
+                            p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].z), __uint_as_float(r[x][c].w)),
+                                                 make_float2(__uint_as_float(b.z), __uint_as_float(b.w)), p[x][j]);
                         }
                     }
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    float h[4];
+                    float f[8], h[4];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = p[x][j].x + p[x][j].y;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float give = t & 2 ? p[x][j] : p[x][j + 4], keep = t & 2 ? p[x][j + 4] : p[x][j];
+                        const float give = t & 2 ? f[j] : f[j + 4], keep = t & 2 ? f[j + 4] : f[j];
                         h[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
                     }
 #pragma unroll
@@ -162,18 +163,14 @@ template <> __device__ __forceinline__ uint4 pack16<__half>(const float* f) {
     return make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]), pack2<__half>(f[4], f[5]), pack2<__half>(f[6], f[7]));
 }
 
-// 16 values of one head in a warp's registers: ROWLANES lanes side by side hold a row, the warp SUBS rows at a time.  The product
-// with the weights stays on float32 FMAs: it has one row of weights per head, a sixteenth of what an mma computes, and the weights
-// would have to be rounded.
-template <typename T, int DMAX> struct ValueTile {
-    static constexpr int EPL = 16 / (int)sizeof(T);
-    static constexpr int ROWLANES = DMAX / EPL;
-    static constexpr int SUBS = 32 / ROWLANES;
-    static constexpr int STEPS = KEYS / SUBS;
+// 16 float32 values of one head in a warp's registers: ROWLANES lanes side by side hold a row, the warp SUBS rows at a time; the
+// product with the weights runs on FMAs.
+template <int DMAX> struct ValueTileF32 {
+    static constexpr int ROWLANES = DMAX / 4, SUBS = 32 / ROWLANES, STEPS = KEYS / SUBS;
     uint4 r[STEPS];
 
-    __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
-        const int sub = lane / ROWLANES, e = (lane % ROWLANES) * EPL;
+    __device__ __forceinline__ void load(const float* pool, long base, int live, int D, int lane) {
+        const int sub = lane / ROWLANES, e = (lane % ROWLANES) * 4;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
             const bool on = base >= 0 && i * SUBS + sub < live && e < D;
@@ -181,6 +178,77 @@ template <typename T, int DMAX> struct ValueTile {
         }
     }
 };
+
+// 16 values of one head in 16 bits as the A operand of mma.sync, transposed: rows are elements, columns keys.  Lane (g, t) loads
+// the 16 bytes at element 64c + 8g of keys 2t, 2t + 1, 2t + 8 and 2t + 9 (8 lanes on 128 contiguous bytes) and pairs neighbouring keys'
+// halves with one byte permute each; mma (c, j) has element 64c + 8g + j as its row g and 64c + 8g + j + 4 as its row g + 8.
+//
+// The B operand's eight columns hold the weights of GT heads, each split into PIECES 16-bit numbers that add up to it: columns
+// y * STRIDE + i, i < PIECES, so that an mma that has eight columns anyway multiplies weights of 24 (bf16) or 33 bits (fp16) with the
+// values at no cost; with four heads two pieces fit, 16 bits or 22, whose rounding of 2^-16 at most is far below the 2^-8 of
+// a bf16 result.  Against FMAs on unpacked values (8 conversions and 4 packed FMAs for 8 elements and head) this takes a half of the
+// instructions for one head, a sixth for four.
+template <int GT> struct Pieces {
+    static constexpr int PIECES = GT == 4 ? 2 : 3, STRIDE = 8 / (GT == 1 ? 2 : GT);
+};
+template <typename T, int DMAX> struct ValueTile {
+    static constexpr int CHUNKS = DMAX / 64;
+    uint4 r[4][CHUNKS];
+
+    __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = 2 * t + (i & 1) + (i >> 1) * 8;
+            const bool on = base >= 0 && key < live;
+            const T* row = pool + (on ? base + (long)key * D : 0);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) {
+                const int e = c * 64 + g * 8;
+                r[i][c] = on && e < D ? __ldg(reinterpret_cast<const uint4*>(row + e)) : make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+    // acc[c][j] += values x weights: [0], [1] element 64c + 8g + j, columns 2t and 2t + 1; [2], [3] element 64c + 8g + j + 4.
+    __device__ __forceinline__ void multiply(float (&acc)[CHUNKS][4][4], uint32_t b0, uint32_t b1) const {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
+                const uint32_t lo[4] = {j < 2 ? r[0][c].x : r[0][c].y, j < 2 ? r[1][c].x : r[1][c].y, j < 2 ? r[2][c].x : r[2][c].y, j < 2 ? r[3][c].x : r[3][c].y};
+                const uint32_t hi[4] = {j < 2 ? r[0][c].z : r[0][c].w, j < 2 ? r[1][c].z : r[1][c].w, j < 2 ? r[2][c].z : r[2][c].w, j < 2 ? r[3][c].z : r[3][c].w};
+                mma_16816<T>(acc[c][j], __byte_perm(lo[0], lo[1], sel), __byte_perm(hi[0], hi[1], sel), __byte_perm(lo[2], lo[3], sel),
+                             __byte_perm(hi[2], hi[3], sel), b0, b1);
+            }
+        }
+    }
+};
+// x as a sum of PIECES numbers of type T, the i-th of them.
+template <typename T, int PIECES> __device__ __forceinline__ void split_pieces(float x, float (&piece)[PIECES]) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        piece[i] = round_to<T>(x);
+        x -= piece[i];
+    }
+}
+
+// Maximum over the warp in one instruction.
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^x to a relative 2^-22; 0 below the smallest normal number.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Brings memory into L2 ahead of its use: 16-byte aligned, a multiple of 16 bytes.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 
 // Work on sequences of different lengths is cut into `workers` equal runs of tiles; a run may begin in one sequence (line) and end
 // in another.  Tile range of worker w of n tiles, and the worker that has tile x.

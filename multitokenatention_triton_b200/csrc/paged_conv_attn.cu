@@ -11,13 +11,18 @@
 // enter a running softmax (maximum, sum and output in float32 registers), and the loads of the next keys and values are issued
 // as soon as the registers of the last ones are free.  Runs are equal cuts of all tiles of all sequences and heads, so lengths need
 // not be alike; a second kernel joins the runs of a head.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace mta {
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int RING = 3 * KEYS, RING_PITCH = RING + 4;   // the pitch spreads an accumulator's rows over the banks
+// Scores stand in pairs of query rows, (row 2i, row 2i + 1) side by side, so that one packed FMA serves two tap rows.
+constexpr int RING = 3 * KEYS, RING_PITCH = 2 * RING + 8;   // floats of a pair of rows; the pitch spreads an accumulator's rows over the banks
+constexpr int P_PITCH = KEYS + 8;                           // 16-bit weights of one column of the product with the values
+constexpr float FP16_WEIGHT = 16384.0f;                     // keeps the pieces of small weights out of fp16's subnormal numbers
 
 struct ConvAttnArgs {
     const void* w;
@@ -35,26 +40,33 @@ __device__ __forceinline__ long workers_of(const ConvAttnArgs& a, long n) {
     return most < a.workers ? most : a.workers;
 }
 
-// GT query heads that share a kv head, NT * 8 >= GT * cq rows of scores.
-template <typename T, int DMAX, int GT, int NT> constexpr size_t conv_attn_warp_smem(int cq, int ck) {
-    return (size_t)NT * 8 * (DMAX * sizeof(T) + 64) + (size_t)NT * 8 * RING_PITCH * 4 + (size_t)GT * cq * ((ck + 3) / 4 * 4) * 4 + GT * KEYS * 4;
+// Blocks that share an SM, by the bytes of a row: what the registers of a tile of keys, one of values and the outputs allow.  One block
+// more at 256 bytes spilled 76 bytes a thread.
+__host__ __device__ constexpr int blocks_per_sm(int row_bytes) { return row_bytes > 256 ? 2 : row_bytes > 128 ? 3 : 4; }
+
+// GT query heads that share a kv head, each with cq rows rounded up to pairs; NT * 8 >= all their rows of scores.
+template <typename T, int DMAX, int GT, int NT> __host__ __device__ constexpr size_t conv_attn_warp_smem(int cq, int ck) {
+    return (size_t)NT * 8 * (DMAX * sizeof(T) + 64) + (size_t)NT * 4 * RING_PITCH * 4 + (size_t)GT * ((cq + 1) / 2) * ((ck + 1) / 2 * 2) * 8 +
+           (sizeof(T) == 2 ? 8 * P_PITCH * 2 : GT * KEYS * 4);
 }
 
 template <typename T, int DMAX, int GT, int NT>
-__global__ void __launch_bounds__(WARPS * 32, sizeof(T) * DMAX > 256 ? 2 : 4) conv_attn_decode_kernel(PagedCache c, ConvAttnArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMAX)) conv_attn_decode_kernel(PagedCache c, ConvAttnArgs a) {
+    constexpr bool HALF = sizeof(T) == 2;
     using K = KeyTile<T, DMAX>;
-    using V = ValueTile<T, DMAX>;
+    using V = std::conditional_t<HALF, ValueTile<T, DMAX>, ValueTileF32<DMAX>>;
+    using P = Pieces<GT>;
     constexpr int EPL = K::EPL;
     extern __shared__ __align__(16) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int ckp = (a.ck + 3) / 4 * 4;
+    const int cqp = (a.cq + 1) / 2, ckp = (a.ck + 1) / 2 * 2;
     char* mine = smem + warp * conv_attn_warp_smem<T, DMAX, GT, NT>(a.cq, a.ck);
     // row pitch of the queries: 64 bytes more than a multiple of 128, so that rows g and g + 1 of an 8-lane phase miss each other's banks
     constexpr int QP = DMAX * (int)sizeof(T) + 64;
     char* q_sm = mine;
     float* s_sm = reinterpret_cast<float*>(mine + NT * 8 * QP);
-    float* w_sm = s_sm + NT * 8 * RING_PITCH;
-    float* p_sm = w_sm + GT * a.cq * ckp;
+    float2* w_sm = reinterpret_cast<float2*>(s_sm + NT * 4 * RING_PITCH);       // [head][pair of tap rows][key tap]
+    T* p_sm = reinterpret_cast<T*>(w_sm + GT * cqp * ckp);                      // [column][key]; float32: [head][key]
     int* before = reinterpret_cast<int*>(smem + WARPS * conv_attn_warp_smem<T, DMAX, GT, NT>(a.cq, a.ck));
     int* lens = before + a.B + 1;
 
@@ -68,7 +80,7 @@ __global__ void __launch_bounds__(WARPS * 32, sizeof(T) * DMAX > 256 ? 2 : 4) co
     const long end = run_begin(me + 1, n, workers);
     const T* k_pool = static_cast<const T*>(c.k);
     const T* v_pool = static_cast<const T*>(c.v);
-    const int left = (a.ck - 1) / 2, shift = left & 3;               // `shift` puts a tile's first window on a 16-byte boundary
+    const int left = (a.ck - 1) / 2, shift = left & 1;               // `shift` puts the window of an even key on a 16-byte boundary
 
     for (long x = run_begin(me, n, workers); x < end;) {
         int b = 0;
@@ -86,139 +98,208 @@ __global__ void __launch_bounds__(WARPS * 32, sizeof(T) * DMAX > 256 ? 2 : 4) co
         const int u1 = (int)(end - x < tiles - u0 ? u0 + (end - x) : tiles);
         const int h0 = line * GT, kv_head = h0 / group;
 
-        // queries and taps of this line
-        for (int i = lane; i < NT * 8 * (DMAX / EPL); i += 32) {
-            const int row = i / (DMAX / EPL), e = (i % (DMAX / EPL)) * EPL, gq = row / a.cq, pos = len - a.cq + row % a.cq;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (gq < GT && pos >= 0 && e < c.D)
-                u = *reinterpret_cast<const uint4*>(static_cast<const T*>(c.q_hist) + (((long)slot * c.ring + pos % c.ring) * c.H + h0 + gq) * c.D + e);
-            *reinterpret_cast<uint4*>(q_sm + row * QP + e * (int)sizeof(T)) = u;
-        }
-        for (int i = lane; i < GT * a.cq * ckp; i += 32) {
-            const int j = i % ckp, row = i / ckp;
-            w_sm[i] = j < a.ck ? load_weight(a.w, ((long)h0 * a.cq + row) * a.ck + j, a.w_dtype) : 0.0f;
-        }
-        __syncwarp();
-
-        float m[GT], l[GT], o[GT][EPL];
-#pragma unroll
-        for (int y = 0; y < GT; ++y) {
-            m[y] = -INFINITY; l[y] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) o[y][e] = 0.0f;
-        }
         K keys;
         V values;
         auto live = [&](int u) { const int r = len - u * KEYS; return r < KEYS ? r : KEYS; };
         auto key_base = [&](int u) { return u >= 0 && u < tiles ? c.at(slot, kv_head, u * KEYS) : -1L; };
         keys.load(k_pool, key_base(u0 - 1), KEYS, c.D, lane);        // a tile before this one is whole
         values.load(v_pool, key_base(u0), live(u0), c.D, lane);
+
+        // queries and taps of this line
+        for (int i = lane; i < NT * 8 * (DMAX / EPL); i += 32) {
+            const int row = i / (DMAX / EPL), e = (i % (DMAX / EPL)) * EPL, gq = row / (2 * cqp), tap = row % (2 * cqp), pos = len - a.cq + tap;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (gq < GT && tap < a.cq && pos >= 0 && e < c.D)
+                u = *reinterpret_cast<const uint4*>(static_cast<const T*>(c.q_hist) + (((long)slot * c.ring + pos % c.ring) * c.H + h0 + gq) * c.D + e);
+            *reinterpret_cast<uint4*>(q_sm + row * QP + e * (int)sizeof(T)) = u;
+        }
+        for (int i = lane; i < GT * cqp * ckp; i += 32) {
+            const int j = i % ckp, pair = i / ckp % cqp, y = i / ckp / cqp;
+            const long at = ((long)(h0 + y) * a.cq + 2 * pair) * a.ck + j;
+            w_sm[i] = make_float2(j < a.ck ? load_weight(a.w, at, a.w_dtype) * a.scale : 0.0f,
+                                  j < a.ck && 2 * pair + 1 < a.cq ? load_weight(a.w, at + a.ck, a.w_dtype) * a.scale : 0.0f);
+        }
+        if constexpr (HALF) {
+            for (int i = lane; i < 8 * P_PITCH / 2; i += 32) reinterpret_cast<uint32_t*>(p_sm)[i] = 0;      // columns that no piece fills
+        }
+        __syncwarp();
+
+        float m[GT], l[GT];                                          // l: this lane's own keys
+        float o[HALF ? DMAX / 64 : GT][4][4];                        // mma accumulators; float32: [head][0][element]
+#pragma unroll
+        for (int y = 0; y < GT; ++y) { m[y] = -INFINITY; l[y] = 0.0f; }
+#pragma unroll
+        for (int i = 0; i < (HALF ? DMAX / 64 : GT); ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+
         for (int u = u0 - 1; u <= u1; ++u) {
             float acc[NT][4];
             keys.template score<NT>(acc, lane, [&](int row, int ch) {
-                return *reinterpret_cast<const uint4*>(q_sm + row * QP + ch * 64 + t4 * 16);
+                return *reinterpret_cast<const uint4*>(q_sm + (HALF ? 8 * row + g : row) * QP + ch * 64 + t4 * 16);
             });
             if (u < u1) keys.load(k_pool, key_base(u + 1), live(u + 1), c.D, lane);
             const int col = ((u + 3) % 3) * KEYS + shift;
+            // scores above the diagonal are zero; those of tiles outside the sequence are zero already
+            if (u * KEYS + KEYS - 1 > len - a.cq) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int row = 8 * nt + 2 * t4 + (y & 1), kk = g + 8 * (y >> 1), key = u * KEYS + kk;
-                    // scores above the diagonal are zero; those of tiles outside the sequence are zero already
-                    const float s = key <= len - a.cq + row % a.cq ? acc[nt][y] : 0.0f;
-                    const int at = col + kk;
-                    s_sm[row * RING_PITCH + (at >= RING ? at - RING : at)] = s;
-                }
+                    for (int y = 0; y < 4; ++y)
+                        if (u * KEYS + g + 8 * (y >> 1) > len - a.cq + (8 * nt + 2 * t4 + (y & 1)) % (2 * cqp)) acc[nt][y] = 0.0f;
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                int at = col + g + 8 * y;
+                if (at >= RING) at -= RING;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    *reinterpret_cast<float2*>(s_sm + (4 * nt + t4) * RING_PITCH + 2 * at) = make_float2(acc[nt][2 * y], acc[nt][2 * y + 1]);
             }
             __syncwarp();
             if (u > u0) {
                 const int un = u - 1;
-                // conv: lane (i, quad) sums tap rows i, i + 8, ... for four keys, then the eight rows are added
+                // conv: lane (i, pair of keys) sums the pairs of tap rows i, i + 4, ...; then the four lanes of a key are added
+                int first = (un % 3) * KEYS + 2 * (lane & 7) + shift - left;       // even
+                if (first < 0) first += RING;
+                float fade[GT];
+                bool moved = false;
 #pragma unroll
                 for (int y = 0; y < GT; ++y) {
-                    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    int first = (un % 3) * KEYS + 4 * t4 + shift - left;           // a multiple of 4
-                    if (first < 0) first += RING;
-                    for (int i = g; i < a.cq; i += 8) {
-                        const float4* srow = reinterpret_cast<const float4*>(s_sm + (y * a.cq + i) * RING_PITCH);
-                        const float4* wrow = reinterpret_cast<const float4*>(w_sm + (y * a.cq + i) * ckp);
-                        int at = first / 4;
+                    float2 z0 = make_float2(0.0f, 0.0f), z1 = z0;
+                    for (int i = lane >> 3; i < cqp; i += 4) {
+                        const float4* srow = reinterpret_cast<const float4*>(s_sm + (y * cqp + i) * RING_PITCH);
+                        const float4* wrow = reinterpret_cast<const float4*>(w_sm + (y * cqp + i) * ckp);
+                        int at = first / 2;
                         float4 lo = srow[at];
-                        for (int j = 0; j < ckp / 4; ++j) {
-                            at = at + 1 == RING / 4 ? 0 : at + 1;
+#pragma unroll 2
+                        for (int j = 0; j < ckp / 2; ++j) {
+                            at = at + 1 == RING / 2 ? 0 : at + 1;
                             const float4 hi = srow[at], w = wrow[j];
-                            z[0] = fmaf(w.x, lo.x, fmaf(w.y, lo.y, fmaf(w.z, lo.z, fmaf(w.w, lo.w, z[0]))));
-                            z[1] = fmaf(w.x, lo.y, fmaf(w.y, lo.z, fmaf(w.z, lo.w, fmaf(w.w, hi.x, z[1]))));
-                            z[2] = fmaf(w.x, lo.z, fmaf(w.y, lo.w, fmaf(w.z, hi.x, fmaf(w.w, hi.y, z[2]))));
-                            z[3] = fmaf(w.x, lo.w, fmaf(w.y, hi.x, fmaf(w.z, hi.y, fmaf(w.w, hi.z, z[3]))));
+                            z0 = __ffma2_rn(make_float2(w.x, w.y), make_float2(lo.x, lo.y), z0);
+                            z1 = __ffma2_rn(make_float2(w.x, w.y), make_float2(lo.z, lo.w), z1);
+                            z0 = __ffma2_rn(make_float2(w.z, w.w), make_float2(lo.z, lo.w), z0);
+                            z1 = __ffma2_rn(make_float2(w.z, w.w), make_float2(hi.x, hi.y), z1);
                             lo = hi;
                         }
                     }
+                    float z[2] = {z0.x + z0.y, z1.x + z1.y}, p[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int s = 4; s < 32; s <<= 1) z[e] += __shfl_xor_sync(0xffffffffu, z[e], s);
-                        z[e] = un * KEYS + 4 * t4 + e < len ? z[e] * a.scale : -INFINITY;
+                    for (int e = 0; e < 2; ++e) {
+                        z[e] += __shfl_xor_sync(0xffffffffu, z[e], 8);
+                        z[e] += __shfl_xor_sync(0xffffffffu, z[e], 16);
+                        if (un * KEYS + 2 * (lane & 7) + e >= len) z[e] = -INFINITY;
                     }
-                    float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float m_new = fmaxf(m[y], top);
+                    const float top = fmaxf(m[y], warp_max(fmaxf(z[0], z[1])));
                     // while every logit so far is -inf nothing has been summed: a finite stand-in keeps -inf - -inf away
-                    const float ref = m_new == -INFINITY ? 0.0f : m_new;
-                    const float fade = exp2f(m[y] - ref);
-                    float sum = 0.0f, p[4];
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    fade[y] = fast_exp2(m[y] - ref);
+                    moved |= top != m[y];
+                    m[y] = top;
+                    p[0] = fast_exp2(z[0] - ref);
+                    p[1] = fast_exp2(z[1] - ref);
+                    l[y] = fmaf(l[y], fade[y], p[0] + p[1]);
+                    if constexpr (HALF) {
+                        constexpr float by = std::is_same_v<T, __half> ? FP16_WEIGHT : 1.0f;
+                        float a0[P::PIECES], a1[P::PIECES];
+                        split_pieces<T>(p[0] * by, a0);
+                        split_pieces<T>(p[1] * by, a1);
+                        // the four lanes that hold these keys write a piece each
+                        float w0 = a0[0], w1 = a1[0];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { p[e] = exp2f(z[e] - ref); sum += p[e]; }
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    l[y] = l[y] * fade + sum;
-                    m[y] = m_new;
-#pragma unroll
-                    for (int e = 0; e < EPL; ++e) o[y][e] *= fade;
-                    if (g == 0) *reinterpret_cast<float4*>(p_sm + y * KEYS + 4 * t4) = make_float4(p[0], p[1], p[2], p[3]);
+                        for (int i = 1; i < P::PIECES; ++i)
+                            if (lane >> 3 == i) { w0 = a0[i]; w1 = a1[i]; }
+                        if (lane >> 3 < P::PIECES)
+                            *reinterpret_cast<uint32_t*>(p_sm + (y * P::STRIDE + (lane >> 3)) * P_PITCH + 2 * (lane & 7)) = pack2<T>(w0, w1);
+                    } else {
+                        if (lane < 8) *reinterpret_cast<float2*>(p_sm + y * KEYS + 2 * lane) = make_float2(p[0], p[1]);
+                    }
                 }
                 __syncwarp();
+                if constexpr (HALF) {
+                    if (moved) {
+                        float f0 = fade[0], f1 = fade[0];
 #pragma unroll
-                for (int i = 0; i < V::STEPS; ++i) {
-                    float f[EPL];
-                    unpack16<T>(values.r[i], f);
+                        for (int y = 1; y < GT; ++y) {
+                            if (2 * t4 / P::STRIDE == y) f0 = fade[y];
+                            if ((2 * t4 + 1) / P::STRIDE == y) f1 = fade[y];
+                        }
 #pragma unroll
-                    for (int y = 0; y < GT; ++y) {
-                        const float p = p_sm[y * KEYS + i * V::SUBS + lane / V::ROWLANES];
+                        for (int i = 0; i < V::CHUNKS; ++i)
 #pragma unroll
-                        for (int e = 0; e < EPL; ++e) o[y][e] = fmaf(p, f[e], o[y][e]);
+                            for (int j = 0; j < 4; ++j) { o[i][j][0] *= f0; o[i][j][1] *= f1; o[i][j][2] *= f0; o[i][j][3] *= f1; }
+                    }
+                    const uint32_t* col_p = reinterpret_cast<const uint32_t*>(p_sm + g * P_PITCH) + t4;
+                    values.multiply(o, col_p[0], col_p[4]);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < GT; ++y)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[y][0][e] *= fade[y];
+#pragma unroll
+                    for (int i = 0; i < V::STEPS; ++i) {
+                        float f[4];
+                        unpack16<float>(values.r[i], f);
+#pragma unroll
+                        for (int y = 0; y < GT; ++y) {
+                            const float p = p_sm[y * KEYS + i * V::SUBS + lane / V::ROWLANES];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[y][0][e] = fmaf(p, f[e], o[y][0][e]);
+                        }
                     }
                 }
                 if (u < u1) values.load(v_pool, key_base(u), live(u), c.D, lane);
             }
             __syncwarp();
         }
+        const bool all = u0 == 0 && u1 == tiles;                     // the whole line: nothing to join
+        const long part = me + (long)b * lines + line;
+        // Stores EPL elements of head y from element e0 on.
+        auto store = [&](int y, int e0, const float* f) {
+            if (all) {
+                float r[EPL];
 #pragma unroll
-        for (int y = 0; y < GT; ++y)
-#pragma unroll
-            for (int e = 0; e < EPL; ++e)
-#pragma unroll
-                for (int s = V::ROWLANES; s < 32; s <<= 1) o[y][e] += __shfl_xor_sync(0xffffffffu, o[y][e], s);
-        const int e0 = (lane % V::ROWLANES) * EPL;
-        if (lane < V::ROWLANES && e0 < c.D) {
-            if (u0 == 0 && u1 == tiles) {                            // the whole line: nothing to join
-#pragma unroll
-                for (int y = 0; y < GT; ++y) {
-#pragma unroll
-                    for (int e = 0; e < EPL; ++e) o[y][e] /= l[y];
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((long)b * c.H + h0 + y) * c.D + e0) = pack16<T>(o[y]);
-                }
+                for (int e = 0; e < EPL; ++e) r[e] = f[e] / l[y];
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((long)b * c.H + h0 + y) * c.D + e0) = pack16<T>(r);
             } else {
-                const long part = me + (long)b * lines + line;
+                float* to = a.part_o + (part * GT + y) * c.D + e0;
 #pragma unroll
-                for (int y = 0; y < GT; ++y) {
-                    float* to = a.part_o + (part * GT + y) * c.D + e0;
+                for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            }
+        };
 #pragma unroll
-                    for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(o[y][e], o[y][e + 1], o[y][e + 2], o[y][e + 3]);
-                    if (lane == 0) a.part_ml[part * GT + y] = make_float2(m[y], l[y]);
+        for (int y = 0; y < GT; ++y) {
+#pragma unroll
+            for (int s = 1; s < 8; s <<= 1) l[y] += __shfl_xor_sync(0xffffffffu, l[y], s);
+            if (lane == 0 && !all) a.part_ml[part * GT + y] = make_float2(m[y], l[y]);
+        }
+        if constexpr (HALF) {
+            constexpr float by = std::is_same_v<T, __half> ? 1.0f / FP16_WEIGHT : 1.0f;
+#pragma unroll
+            for (int i = 0; i < V::CHUNKS; ++i) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[j] = (o[i][j][0] + o[i][j][1]) * by;
+                    f[j + 4] = (o[i][j][2] + o[i][j][3]) * by;
                 }
+                if constexpr (P::STRIDE == 4) {                      // a head's columns are those of two lanes
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] += __shfl_xor_sync(0xffffffffu, f[e], 1);
+                }
+                const int e0 = i * 64 + g * 8;
+#pragma unroll
+                for (int y = 0; y < GT; ++y)
+                    if (t4 == y * P::STRIDE / 2 && e0 < c.D) store(y, e0, f);
+            }
+        } else {
+#pragma unroll
+            for (int y = 0; y < GT; ++y) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int s = V::ROWLANES; s < 32; s <<= 1) o[y][0][e] += __shfl_xor_sync(0xffffffffu, o[y][0][e], s);
+                if (lane < V::ROWLANES && lane * 4 < c.D) store(y, lane * 4, o[y][0]);
             }
         }
         x += u1 - u0;
@@ -281,10 +362,11 @@ template <typename T> __global__ void __launch_bounds__(128) conv_attn_join_kern
 
 constexpr int MIN_TILES = 4;
 
-// Query heads that a warp takes together: all that share a kv head if the scores of at most four fit in 32 rows.
+// Query heads that a warp takes together: up to four that share a kv head, if their scores, an even number of rows each, fit in 32 rows.
 int heads_together(int group, int cq) {
-    if (group % 4 == 0 && 4 * cq <= DECODE_MAX_ROWS) return 4;
-    if (group % 2 == 0 && 2 * cq <= DECODE_MAX_ROWS) return 2;
+    const int rows = (cq + 1) / 2 * 2;
+    if (group % 4 == 0 && 4 * rows <= DECODE_MAX_ROWS) return 4;
+    if (group % 2 == 0 && 2 * rows <= DECODE_MAX_ROWS) return 2;
     return 1;
 }
 
@@ -293,16 +375,20 @@ struct Plan {
     size_t ml_bytes, bytes;
 };
 
-Plan make_plan(int B, int H, int kv_heads, int D, int cq, int max_length) {
+// Room for as many runs as there can be for any type; `row_bytes` (0: not known) sets the number of this call's.
+Plan make_plan(int B, int H, int kv_heads, int D, int cq, int max_length, int row_bytes) {
     Plan plan, *p = &plan;
     p->gt = heads_together(H / kv_heads, cq);
     const long lines = (long)B * (H / p->gt), tiles = lines * ((max_length + KEYS - 1) / KEYS);
     long workers = (tiles + MIN_TILES - 1) / MIN_TILES;
-    const long most = (long)DECODE_SMS * 16;
-    p->workers = (int)(workers < most ? (workers < 1 ? 1 : workers) : most);
-    const size_t parts = (size_t)(p->workers + lines) * p->gt;
+    const long most = (long)DECODE_SMS * WARPS * blocks_per_sm(0);
+    if (workers > most) workers = most;
+    if (workers < 1) workers = 1;
+    const size_t parts = (size_t)(workers + lines) * p->gt;
     p->ml_bytes = (parts * sizeof(float2) + 255) / 256 * 256;
     p->bytes = p->ml_bytes + parts * D * sizeof(float);
+    const long wave = (long)DECODE_SMS * WARPS * blocks_per_sm(row_bytes);
+    p->workers = (int)(workers < wave ? workers : wave);
     return plan;
 }
 
@@ -315,7 +401,7 @@ int launch(const PagedCache& c, const ConvAttnArgs& a, cudaStream_t st) {
 }
 
 template <typename T, int DMAX> int launch_rows(const PagedCache& c, const ConvAttnArgs& a, int gt, cudaStream_t st) {
-    const int nt = (gt * a.cq + 7) / 8;
+    const int nt = (gt * ((a.cq + 1) / 2 * 2) + 7) / 8;
     if (gt == 4) return nt <= 3 ? launch<T, DMAX, 4, 3>(c, a, st) : launch<T, DMAX, 4, 4>(c, a, st);
     if (gt == 2) return nt <= 2 ? launch<T, DMAX, 2, 2>(c, a, st) : launch<T, DMAX, 2, 4>(c, a, st);
     return nt <= 1 ? launch<T, DMAX, 1, 1>(c, a, st) : nt <= 2 ? launch<T, DMAX, 1, 2>(c, a, st) : launch<T, DMAX, 1, 4>(c, a, st);
@@ -330,14 +416,14 @@ template <typename T> int launch_dim(const PagedCache& c, const ConvAttnArgs& a,
 }  // namespace
 
 size_t conv_attn_decode_workspace(int B, int H, int kv_heads, int D, int cq, int max_length) {
-    return make_plan(B, H, kv_heads, D, cq, max_length).bytes;
+    return make_plan(B, H, kv_heads, D, cq, max_length, 0).bytes;
 }
 
 int conv_attn_decode_launch(const PagedCache& cache, const void* w, int w_dtype, void* out, void* workspace, int B, int cq, int ck, float scale, int dtype,
                             cudaStream_t st) {
     PagedCache c = cache;
     if (int rc = wait_flag_ptr(&c.err)) return rc;
-    const Plan p = make_plan(B, c.H, c.kv_heads, c.D, cq, c.max_length);
+    const Plan p = make_plan(B, c.H, c.kv_heads, c.D, cq, c.max_length, (c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256) * (int)dtype_size(dtype));
     ConvAttnArgs a;
     a.w = w; a.w_dtype = w_dtype; a.out = out; a.B = B; a.cq = cq; a.ck = ck; a.scale = scale * LOG2E;
     a.part_ml = static_cast<float2*>(workspace);

@@ -3,11 +3,14 @@
 The bound follows the computation: every sum of n products done in float32 is off by at most n * U times the sum of the products'
 magnitudes (U = 2^-22: four roundings' worth for each, which covers the alignment inside a tensor core's accumulator), errors of
 inputs pass through the linear stages with the weights' magnitudes, and a probability's relative error is at most twice the largest
-error of the row's logits plus the roundings of the exponent and of the sum.
+error of the row's logits plus the roundings of the exponent and of the sum.  With 16-bit values the kernels may multiply them with
+weights that are sums of two numbers of that type: the first is off by half a step, the second by half a step of that, 2^-16 in bf16
+and 2^-22 in fp16, where a number scaled to 2^15 at most is also off by half of 2^-24, 2^-39 of the largest weight.
 """
 import torch
 
 U = 2.0 ** -22
+PIECES = {torch.float32: 0.0, torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -16}
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
@@ -27,6 +30,7 @@ def conv64(x, w):
 def token64(q, k, v, w1, scale, W1=None, w2=None, W2=None):
     """The newest token of one sequence: q (H,n,D) all its queries, k, v (kv heads,n,D), the weights; all taken to float64.  Returns
     (out (H,D), bound on the absolute error of a float32 evaluation).  Without W1, w2 and W2 the conv attention."""
+    dtype = q.dtype
     q, k, v, w1 = q.double(), k.double(), v.double(), w1.double()
     H, n, D = q.shape
     k, v = (t.repeat_interleave(H // t.shape[0], 0) for t in (k, v))
@@ -54,6 +58,9 @@ def token64(q, k, v, w1, scale, W1=None, w2=None, W2=None):
         y, ey = conv64(p, w2), conv64(ep, w2.abs()) + conv64(p, w2.abs()) * (w2[0].numel() + 1) * U
         p = torch.tensordot(W2, y, dims=1)
         ep = torch.tensordot(W2.abs(), ey + y.abs() * (H + 1) * U, dims=1)
+    ep = ep + p.abs() * PIECES[dtype]
+    if dtype == torch.float16:
+        ep = ep + 2.0 ** -39 * (1.0 if W1 is None else (W2.abs() @ w2.abs().sum((1, 2)))[:, None, None])
     out = (p @ v)[:, 0]
     return out, (ep @ v.abs() + (p.abs() @ v.abs()) * (n + 8) * U)[:, 0]
 
