@@ -61,9 +61,18 @@ template <typename T, int DMAX> struct KeyTile {
     static constexpr int EPL = 16 / (int)sizeof(T);      // elements in 16 bytes
     uint4 r[2][CH];
 
-    // Rows base, base + 1, ... of which `live` exist; the others are zero and not read.  base < 0: none exists.
+    // Rows base, base + 1, ... of which `live` exist; the others are zero and not read.  base < 0: none exists.  The usual whole tile
+    // takes a path of plain loads: setting the registers to zero first costs as much as everything else here.
     __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
         const int g = lane >> 2, t = lane & 3;
+        if (base >= 0 && live >= KEYS && D == DMAX) {
+            const T* row = pool + base + (g * DMAX + t * EPL);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) r[x][c] = __ldg(reinterpret_cast<const uint4*>(row + x * 8 * DMAX + c * 4 * EPL));
+            return;
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const bool on = base >= 0 && g + 8 * x < live;
@@ -71,7 +80,8 @@ template <typename T, int DMAX> struct KeyTile {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int e = (c * 4 + t) * EPL;
-                r[x][c] = on && e < D ? __ldg(reinterpret_cast<const uint4*>(row + e)) : make_uint4(0, 0, 0, 0);
+                r[x][c] = make_uint4(0, 0, 0, 0);
+                if (on && e < D) r[x][c] = __ldg(reinterpret_cast<const uint4*>(row + e));
             }
         }
     }
@@ -91,42 +101,44 @@ template <typename T, int DMAX> struct KeyTile {
                 }
             }
         } else {
-            // float32 on FMAs: each lane sums its quarter of the elements for eight rows, then the four lanes of a key exchange
-            // halves twice, which leaves every lane with the two rows that the mma layout gives it
+            // float32 on FMAs: each lane sums its quarter of the elements for four rows at a time, then the four lanes of a key add up
+            // and share out the rows, so that every lane has the two that the mma layout gives it
             const int t = lane & 3;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float2 p[2][8];                              // sums of even and odd elements
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[0][j] = p[1][j] = make_float2(0.0f, 0.0f);
+                for (int half = 0; half < 2; ++half) {
+                    float2 p[2][4];                          // sums of even and odd elements
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
+                    for (int j = 0; j < 4; ++j) p[0][j] = p[1][j] = make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint4 b = q(8 * n + j, c);
+                    for (int c = 0; c < CH; ++c) {
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].x), __uint_as_float(r[x][c].y)),
-                                                 make_float2(__uint_as_float(b.x), __uint_as_float(b.y)), p[x][j]);
-                            p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].z), __uint_as_float(r[x][c].w)),
-                                                 make_float2(__uint_as_float(b.z), __uint_as_float(b.w)), p[x][j]);
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 b = q(8 * n + 4 * half + j, c);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].x), __uint_as_float(r[x][c].y)),
+                                                     make_float2(__uint_as_float(b.x), __uint_as_float(b.y)), p[x][j]);
+                                p[x][j] = __ffma2_rn(make_float2(__uint_as_float(r[x][c].z), __uint_as_float(r[x][c].w)),
+                                                     make_float2(__uint_as_float(b.z), __uint_as_float(b.w)), p[x][j]);
+                            }
                         }
                     }
-                }
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float f[8], h[4];
+                    for (int x = 0; x < 2; ++x) {
+                        float f[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) f[j] = p[x][j].x + p[x][j].y;
+                        for (int j = 0; j < 4; ++j) {
+                            f[j] = p[x][j].x + p[x][j].y;
+                            f[j] += __shfl_xor_sync(0xffffffffu, f[j], 2);
+                        }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float give = t & 2 ? f[j] : f[j + 4], keep = t & 2 ? f[j + 4] : f[j];
-                        h[j] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float give = t & 1 ? h[j] : h[j + 2], keep = t & 1 ? h[j + 2] : h[j];
-                        acc[n][2 * x + j] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+                        for (int j = 0; j < 2; ++j) {
+                            const float give = t & 1 ? f[j] : f[j + 2], keep = t & 1 ? f[j + 2] : f[j];
+                            const float sum = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+                            if (t >> 1 == half) acc[n][2 * x + j] = sum;
+                        }
                     }
                 }
             }
@@ -171,10 +183,16 @@ template <int DMAX> struct ValueTileF32 {
 
     __device__ __forceinline__ void load(const float* pool, long base, int live, int D, int lane) {
         const int sub = lane / ROWLANES, e = (lane % ROWLANES) * 4;
+        if (base >= 0 && live >= KEYS && D == DMAX) {
+            const float* row = pool + base + (sub * DMAX + e);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) r[i] = __ldg(reinterpret_cast<const uint4*>(row + i * SUBS * DMAX));
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            const bool on = base >= 0 && i * SUBS + sub < live && e < D;
-            r[i] = on ? __ldg(reinterpret_cast<const uint4*>(pool + base + (long)(i * SUBS + sub) * D + e)) : make_uint4(0, 0, 0, 0);
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (base >= 0 && i * SUBS + sub < live && e < D) r[i] = __ldg(reinterpret_cast<const uint4*>(pool + base + (long)(i * SUBS + sub) * D + e));
         }
     }
 };
@@ -197,6 +215,14 @@ template <typename T, int DMAX> struct ValueTile {
 
     __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
         const int g = lane >> 2, t = lane & 3;
+        if (base >= 0 && live >= KEYS && D == DMAX) {
+            const T* row = pool + base + (2 * t * DMAX + g * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) r[i][c] = __ldg(reinterpret_cast<const uint4*>(row + ((i & 1) + (i >> 1) * 8) * DMAX + c * 64));
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = 2 * t + (i & 1) + (i >> 1) * 8;
@@ -205,7 +231,8 @@ template <typename T, int DMAX> struct ValueTile {
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
                 const int e = c * 64 + g * 8;
-                r[i][c] = on && e < D ? __ldg(reinterpret_cast<const uint4*>(row + e)) : make_uint4(0, 0, 0, 0);
+                r[i][c] = make_uint4(0, 0, 0, 0);
+                if (on && e < D) r[i][c] = __ldg(reinterpret_cast<const uint4*>(row + e));
             }
         }
     }
@@ -277,6 +304,11 @@ __device__ __forceinline__ void count_tiles(const PagedCache& c, int B, int shif
         if (lane == 0) before[0] = 0;
     }
 }
+
+// Named barriers between warps of a block that hand work on: `n` threads, those that arrive and those that wait.  Both order the memory
+// accesses before them.  Every call is reached by whole warps; the two sides count the same stages, so that every wait ends.
+__device__ __forceinline__ void barrier_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void barrier_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // The last index b with before[b] <= x, x < before[B].
 __device__ __forceinline__ int find_line(const int* before, int B, long x) {

@@ -21,7 +21,12 @@
 namespace mta {
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+// A block is one per SM, half of its warps on memory and half on arithmetic: eight stream keys (values) and multiply, eight run the
+// convs, head mixes and softmaxes of the tile before (after).  With all sixteen doing one after the other memory stood still for a third of
+// the time: 770 us for 16 sequences of 8192 tokens and 32 heads.
+constexpr int ROLE_WARPS = 8, ROLE_THREADS = ROLE_WARPS * 32, THREADS = 2 * ROLE_THREADS;
+// Named barriers: a stage's buffer is full or empty (by the stage's parity), and those of one half alone.
+enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_MATH = 5, BAR_MEMORY = 6 };
 
 struct MtaArgs {
     const void *w1, *W1, *w2, *W2;
@@ -32,21 +37,22 @@ struct MtaArgs {
     long pitch;
     int w_dtype, B, cq, ck, cq2, ck2;
     float scale;           // log2(e) / sqrt(D), taken into the first conv's taps: logits are in base 2
-    int workers, shift;    // key tiles of 1 << shift
+    int workers, shift;    // tiles of 1 << shift keys; runs are cut between any 16
     int kv_together;       // kv heads whose scores fit in shared memory at once
 };
 
 __host__ __device__ inline int round4(int x) { return (x + 3) / 4 * 4; }
 __host__ __device__ inline int halo(int x) { return (x + KEYS - 1) / KEYS * KEYS; }
 
-// The scores of a tile and its neighbours: a ring of `keys` positions, so that what two tiles share is computed once.  Two heads
-// stand side by side, which lets one packed FMA serve both.  Keys (4i, 4i + 1) lie in the first half of a row, (4i + 2, 4i + 3) in
-// the second, 16 bytes each: the conv's threads, four keys apart, read neighbouring 16 bytes.  The pads put the rows and halves that an
-// accumulator writes at once into different banks.
+// The scores of two tiles and their neighbours: a ring of `keys` positions, so that one tile's scores are written while the conv reads
+// the other's, and what tiles share is computed once; keys lie at their number plus a multiple of 16 that lets a sequence begin
+// where the one before ended.  Where not all heads fit, the tiles (of one group of heads after another) have a ring each.  Two heads stand side by side, which lets one packed FMA serve both.  Keys (4i, 4i + 1) lie in the first half of a
+// row, (4i + 2, 4i + 3) in the second, 16 bytes each: the conv's threads, four keys apart, read neighbouring 16 bytes.  The pads
+// put the rows and halves that an accumulator writes at once into different banks.
 struct ScoreRing {
     int keys, half, row;   // floats of half a row and of a row
-    __host__ __device__ ScoreRing(int tile, int ck) {
-        keys = halo((ck - 1) / 2) + tile + halo(ck - 1 - (ck - 1) / 2);
+    __host__ __device__ ScoreRing(int tile, int ck, bool whole) {
+        keys = (halo((ck - 1) / 2) + tile + halo(ck - 1 - (ck - 1) / 2)) * (whole ? 2 : 1);
         half = keys + (keys % 32 == 0 ? 8 : 24);
         row = 2 * half + 8;
     }
@@ -54,18 +60,20 @@ struct ScoreRing {
 __host__ __device__ inline int prob_pitch(int tile, int ck2) { return tile + round4(ck2) + 4; }
 
 struct ScoreSmem {
-    size_t s, c, W, taps, ml, q_at, before, bytes;
+    size_t s, s_one, c, W, taps, ml, q_at, before, bytes;
 };
-__host__ __device__ inline ScoreSmem score_smem(int B, int H, int group, int kv_together, int tile, int cq, int ck, int cq2) {
+__host__ __device__ inline ScoreSmem score_smem(int B, int H, int group, int kv_heads, int kv_together, int tile, int cq, int ck, int cq2) {
     ScoreSmem m;
     size_t at = 0;
     const int R = cq + cq2 - 1;
-    m.s = at; at += (size_t)((kv_together * group + 1) / 2) * R * ScoreRing(tile, ck).row * 4;
+    const bool whole = kv_together == kv_heads;
+    m.s_one = (size_t)((kv_together * group + 1) / 2) * R * ScoreRing(tile, ck, whole).row * 4;
+    m.s = at; at += m.s_one * (whole ? 1 : 2);
     m.c = at; at += (size_t)cq2 * H * tile * 4;
     m.W = at; at += (size_t)H * round4(H) * 4;
     m.taps = at; at += (size_t)((H + 1) / 2) * cq * round4(ck) * 8;
-    m.ml = at; at += ((size_t)cq2 * H * 8 + 15) / 16 * 16;
-    m.q_at = at; at += DECODE_MAX_ROWS * 8;
+    m.ml = at; at += (size_t)cq2 * H * (tile / 4) * 8;
+    m.q_at = at; at += (size_t)ROLE_WARPS * DECODE_MAX_ROWS * 8;
     m.before = at; at += (size_t)(2 * B + 1) * 4;
     m.bytes = at;
     return m;
@@ -73,17 +81,19 @@ __host__ __device__ inline ScoreSmem score_smem(int B, int H, int group, int kv_
 // 16-bit pieces of the weights in a row of `tile` keys; the pad spreads eight rows over the banks.
 __host__ __device__ inline int piece_pitch(int tile) { return tile + 8; }
 struct ValueSmem {
-    size_t p, y, a, W, taps, ml, by, o, before, bytes;
+    size_t p, y, a, a_one, W, taps, run_taps, ml, by, o, before, bytes;
 };
 __host__ __device__ inline ValueSmem value_smem(int B, int H, int D, int tile, int cq2, int ck2, int copies) {
     ValueSmem m;
     size_t at = 0;
     m.p = at; at += (size_t)cq2 * H * prob_pitch(tile, ck2) * 4;
     m.y = at; at += (size_t)H * tile * 4;
-    m.a = at; at += (size_t)H * (3 * piece_pitch(tile) * 2);     // up to three pieces; float32: 4 bytes a key
+    m.a_one = (size_t)H * (3 * piece_pitch(tile) * 2);           // up to three pieces; float32: 4 bytes a key
+    m.a = at; at += 2 * m.a_one;
     m.W = at; at += (size_t)H * round4(H) * 4;
     m.taps = at; at += (size_t)H * cq2 * round4(ck2) * 4;
-    m.ml = at; at += ((size_t)cq2 * H * 8 + 15) / 16 * 16;
+    m.run_taps = at; at += (size_t)H * cq2 * round4(ck2) * 4;
+    m.ml = at; at += ((size_t)cq2 * H * 4 + 15) / 16 * 16;
     m.by = at; at += (size_t)round4(H) * 4;
     m.o = at; at += (size_t)copies * H * D * 4;
     m.before = at; at += (size_t)(2 * B + 1) * 4;
@@ -94,7 +104,7 @@ __host__ __device__ inline ValueSmem value_smem(int B, int H, int D, int tile, i
 // W transposed to [h][o], so that four outputs are one 16-byte load.
 __device__ __forceinline__ void load_mix(float* W, const void* from, int H, int w_dtype) {
     const int Hp = round4(H);
-    for (int i = threadIdx.x; i < H * Hp; i += THREADS) {
+    for (int i = threadIdx.x % ROLE_THREADS; i < H * Hp; i += ROLE_THREADS) {
         const int o = i / H, h = i - o * H;                      // neighbouring threads read neighbouring weights
         W[h * Hp + o] = o < H ? load_weight(from, (long)o * H + h, w_dtype) : 0.0f;
     }
@@ -131,22 +141,44 @@ __device__ __forceinline__ void mix_heads(float (&z)[4][4], const float* W, cons
     }
 }
 
-// Asks L2 for the rows of `tile` keys of every kv head from key k0 on: 16 keys a thread.
-template <typename T> __device__ __forceinline__ void prefetch_tile(const PagedCache& c, const T* pool, int slot, int k0, int tile, int len) {
-    const int units = tile / KEYS;
-    for (int i = threadIdx.x; i < c.kv_heads * units; i += THREADS) {
-        const int key = k0 + i % units * KEYS;
-        if (key >= len) continue;
-        const long base = c.at(slot, i / units, key);
-        if (base >= 0) prefetch_l2(pool + base, (uint32_t)((len - key < KEYS ? len - key : KEYS) * c.D * sizeof(T)));
-    }
+// Keys [k0, k1) of a sequence, of one block's run.
+struct Span {
+    int b, len, slot, k0, k1;
+};
+// The span that begins with unit x (16 keys) of a run that ends with unit `end`.
+__device__ __forceinline__ Span span_at(const PagedCache& c, const int* before, const int* lens, int B, long x, long end) {
+    Span s;
+    s.b = find_line(before, B, x);
+    s.len = lens[s.b];
+    s.slot = c.slot(s.b);
+    s.k0 = (int)(x - before[s.b]) * KEYS;
+    s.k1 = (int)(end < before[s.b + 1] ? end - before[s.b] : before[s.b + 1] - before[s.b]) * KEYS;
+    return s;
 }
 
-// Blocks an SM: one where two would spill registers (wide rows, many query rows, float32 with more than eight rows).
-__host__ __device__ constexpr int scores_blocks(int elem, int dmax, int nt) { return elem * dmax > 256 || nt == 4 || (elem == 4 && nt > 1) ? 1 : 2; }
+// What is added to key numbers for their places in the ring: key `first` comes to place `to` (a multiple of 16 each), no place is negative.
+__device__ __forceinline__ int ring_turn(const ScoreRing& ring, bool whole, int to, int first) {
+    if (!whole) { to = 0; }
+    int turn = (to - first) % ring.keys;
+    if (turn < 0) turn += ring.keys;
+    return first + turn < 0 ? turn + ring.keys : turn;
+}
+
+// Where the 16 keys of lane `unit` of a stage lie for kv head 0; pages are looked up one stage ahead of their use.
+struct Pages {
+    int page;
+    __device__ void look_up(const PagedCache& c, int slot, int key, bool on) {
+        page = on ? __ldg(c.table + (long)slot * c.table_width + (key >> c.page_shift)) : -1;
+    }
+    __device__ long at(const PagedCache& c, int key, bool on) const {
+        if (!on) return -1;
+        if ((unsigned)page >= (unsigned)c.pages) { c.bad(); return -1; }
+        return ((((long)page * c.kv_heads) << c.page_shift) + (key & ((1 << c.page_shift) - 1))) * c.D;
+    }
+};
 
 template <typename T, int DMAX, int NT>
-__global__ void __launch_bounds__(THREADS, scores_blocks((int)sizeof(T), DMAX, NT)) mta_decode_scores_kernel(PagedCache c, MtaArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCache c, MtaArgs a) {
     constexpr bool HALF = sizeof(T) == 2;
     using K = KeyTile<T, DMAX>;
     extern __shared__ __align__(16) char smem[];
@@ -154,120 +186,221 @@ __global__ void __launch_bounds__(THREADS, scores_blocks((int)sizeof(T), DMAX, N
     const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = round4(a.ck);
     const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo(a.ck - 1 - left);
     const int shift = left & 3;                                  // puts the windows of a tile's quads of keys on 16-byte boundaries
-    const ScoreRing ring(tile, a.ck);
-    const ScoreSmem m = score_smem(a.B, H, group, a.kv_together, tile, a.cq, a.ck, a.cq2);
+    const bool whole = a.kv_together == c.kv_heads;              // all heads at once: what tiles share stays in the ring
+    const ScoreRing ring(tile, a.ck, whole);
+    const ScoreSmem m = score_smem(a.B, H, group, c.kv_heads, a.kv_together, tile, a.cq, a.ck, a.cq2);
     float *s_sm = reinterpret_cast<float*>(smem + m.s), *c_sm = reinterpret_cast<float*>(smem + m.c), *W_sm = reinterpret_cast<float*>(smem + m.W);
+    const int s_other = whole ? 0 : (int)(m.s_one / 4);          // from one stage's ring to the next one's
     float2 *t_sm = reinterpret_cast<float2*>(smem + m.taps), *ml = reinterpret_cast<float2*>(smem + m.ml);
-    long* q_at = reinterpret_cast<long*>(smem + m.q_at);
     int *before = reinterpret_cast<int*>(smem + m.before), *lens = before + a.B + 1;
 
+    // positions that hold no score yet are read with taps of zero, or for keys behind the run: they have to be finite
+    for (int i = threadIdx.x; i < (int)((m.c - m.s) / 16); i += THREADS) reinterpret_cast<float4*>(s_sm)[i] = make_float4(0, 0, 0, 0);
     pdl_wait();
-    count_tiles(c, a.B, a.shift, before, lens);
+    count_tiles(c, a.B, 4, before, lens);
+    __syncthreads();
+    const long n = before[a.B], workers = n < a.workers ? n : a.workers, me = blockIdx.x;
+    if (me >= workers) return;
+    const long begin = run_begin(me, n, workers), end = run_begin(me + 1, n, workers);
+
+    if (warp < ROLE_WARPS) {
+        // ---- scores.  A stage is a tile and a group of heads; a task one kv head and 16 keys of it.
+        const T* pool = static_cast<const T*>(c.k);
+        const T* queries = static_cast<const T*>(c.q_hist);
+        long* q_at = reinterpret_cast<long*>(smem + m.q_at) + warp * DECODE_MAX_ROWS;       // this warp's query rows
+        // Where the loads are: one task ahead of the arithmetic.  Of the tasks behind that, L2 is asked a stage ahead.
+        struct Cursor {
+            Span s;
+            long at;           // of this lane's unit
+            int k0, hk0, first, units, hk, unit, tasks_left, taken, stage, turn;
+            Pages next;
+            bool done;
+        } cur = {};
+        auto first_of = [&](int k0) { return k0 + (whole && k0 > cur.s.k0 ? hr : -hl); };
+        auto units_of = [&](int k0) { return ((k0 + tile < cur.s.k1 ? k0 + tile : cur.s.k1) + hr - first_of(k0)) / KEYS; };
+        // L2 is asked for this warp's tasks of the tile at k0, a task per lane; `at` is the place of the lane's unit.
+        auto ask_l2 = [&](int k0, long at) {
+            const int units = units_of(k0), nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together;
+            const int t0 = warp * nk * units / ROLE_WARPS, t1 = (warp + 1) * nk * units / ROLE_WARPS;
+            for (int t = t0; t < t1; t += 32) {
+                const int mine = t + lane < t1 ? t + lane : t1 - 1, hk = mine / units, unit = mine - hk * units;
+                const long base = __shfl_sync(0xffffffffu, at, unit);
+                const int live = cur.s.len - (first_of(k0) + unit * KEYS);
+                if (t + lane < t1 && base >= 0)
+                    prefetch_l2(pool + base + ((long)(cur.hk0 + hk) << c.page_shift) * c.D, (uint32_t)((live < KEYS ? live : KEYS) * c.D * sizeof(T)));
+            }
+        };
+        auto enter_stage = [&] {
+            cur.first = first_of(cur.k0);
+            cur.units = units_of(cur.k0);
+            const int nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together, tasks = nk * cur.units;
+            const int t0 = warp * tasks / ROLE_WARPS;
+            cur.tasks_left = (warp + 1) * tasks / ROLE_WARPS - t0;
+            cur.taken = 0;
+            cur.hk = t0 / cur.units;
+            cur.unit = t0 - cur.hk * cur.units;
+            const int key = cur.first + lane * KEYS;
+            const bool on = lane < cur.units && key >= 0 && key < cur.s.len;
+            if (!whole || cur.k0 == cur.s.k0) cur.next.look_up(c, cur.s.slot, key, on);
+            cur.at = cur.next.at(c, key, on);
+            if (!whole || cur.k0 == cur.s.k0) ask_l2(cur.k0, cur.at);
+            if (whole) {                                         // the next tile of the span
+                const int ahead = cur.k0 + tile + hr + lane * KEYS;
+                cur.next.look_up(c, cur.s.slot, ahead, lane < tile / KEYS && ahead < cur.s.len);
+            }
+        };
+        auto enter_span = [&](long x, int place) {
+            cur.s = span_at(c, before, lens, a.B, x, end);
+            cur.k0 = cur.s.k0;
+            cur.hk0 = 0;
+            cur.turn = ring_turn(ring, whole, place, cur.s.k0 - hl);
+        };
+        enter_span(begin, 0);
+        enter_stage();
+        K keys;
+        int key = 0, hk = 0;                                     // of the task whose keys are on their way
+        auto fetch = [&]() -> bool {
+            while (!cur.done && cur.tasks_left == 0) {
+                ++cur.stage;
+                cur.hk0 += a.kv_together;
+                if (cur.hk0 >= c.kv_heads) {
+                    cur.hk0 = 0;
+                    cur.k0 += tile;
+                    if (cur.k0 >= cur.s.k1) {
+                        const long x = (long)before[cur.s.b] + cur.s.k1 / KEYS;
+                        if (x >= end) { cur.done = true; break; }
+                        enter_span(x, cur.k0 + hr + cur.turn);   // behind the places of the span's last tile
+                    }
+                }
+                enter_stage();
+            }
+            if (cur.done) return false;
+            const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
+            key = cur.first + cur.unit * KEYS;
+            hk = cur.hk0 + cur.hk;
+            keys.load(pool, base < 0 ? base : base + ((long)hk << c.page_shift) * c.D, cur.s.len - key, c.D, lane);
+            if (++cur.unit == cur.units) { cur.unit = 0; ++cur.hk; }
+            --cur.tasks_left;
+            if (++cur.taken == 2 && whole && cur.k0 + tile < cur.s.k1) {
+                const int ahead = cur.k0 + tile + hr + lane * KEYS;
+                ask_l2(cur.k0 + tile, cur.next.at(c, ahead, lane < tile / KEYS && ahead < cur.s.len));
+            }
+            return true;
+        };
+        int stage = 0, span_b = -1, q_head = -1;
+        uint4 q[HALF ? NT : 1][HALF ? K::CH : 1];
+        for (bool more = fetch(); more;) {
+            // the cursor still stands where this task's keys were fetched
+            while (stage < cur.stage) {
+                barrier_arrive(BAR_FULL + (stage & 1), THREADS);
+                ++stage;
+                if (stage >= 2) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
+            }
+            const int len = cur.s.len;
+            if (cur.s.b != span_b) {
+                __syncwarp();
+                const int pos = len - R + lane;
+                q_at[lane] = lane < R && pos >= 0 ? ((long)cur.s.slot * c.ring + pos % c.ring) * H * c.D : -1;
+                span_b = cur.s.b;
+                q_head = -1;
+                __syncwarp();
+            }
+            const bool full = key + KEYS - 1 <= len - R;                             // every row sees every key
+            const int now = key, local = (hk - cur.hk0) * group, head0 = hk * group;
+            const int at = (now + cur.turn + shift) % ring.keys + g;                 // ring position of key `g` of the unit
+            float* buf = s_sm + (stage & 1) * s_other + 2 * t4 * ring.row;
+            for (int gq = 0; gq < group; ++gq) {
+                const T* qh = queries + (long)(head0 + gq) * c.D;
+                float acc[NT][4];
+                if constexpr (HALF) {
+                    if (q_head != head0 + gq) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const long row = q_at[8 * nt + g];
+#pragma unroll
+                            for (int ch = 0; ch < K::CH; ++ch) {
+                                const int e = (ch * 4 + t4) * K::EPL;
+                                q[nt][ch] = make_uint4(0, 0, 0, 0);
+                                if (row >= 0 && e < c.D) q[nt][ch] = __ldg(reinterpret_cast<const uint4*>(qh + row + e));
+                            }
+                        }
+                        q_head = head0 + gq;
+                    }
+                    keys.template score<NT>(acc, lane, [&](int nt, int ch) { return q[nt][ch]; });
+                } else {
+                    keys.template score<NT>(acc, lane, [&](int row, int ch) {
+                        const long r = q_at[row];
+                        const int e = (ch * 4 + t4) * K::EPL;
+                        return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
+                    });
+                }
+                if (gq == group - 1) more = fetch();
+                float* s = buf + ((local + gq) >> 1) * R * ring.row + ((local + gq) & 1);
+                if (!full) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            if (now + g + 8 * (y >> 1) > len - R + 8 * nt + 2 * t4 + (y & 1)) acc[nt][y] = 0.0f;
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    int pos = at + 8 * y;
+                    if (pos >= ring.keys) pos -= ring.keys;
+                    float* to = s + (pos & ~3) + (pos & 1) * 2 + (pos & 2 ? ring.half : 0);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (8 * nt + 2 * t4 < R) to[8 * nt * ring.row] = acc[nt][2 * y];
+                        if (8 * nt + 2 * t4 + 1 < R) to[(8 * nt + 1) * ring.row] = acc[nt][2 * y + 1];
+                    }
+                }
+            }
+        }
+        // stages behind this warp's last task: the cursor stands behind the run's last stage
+        while (stage < cur.stage) {
+            barrier_arrive(BAR_FULL + (stage & 1), THREADS);
+            ++stage;
+            if (stage >= 2 && stage < cur.stage) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
+        }
+        return;
+    }
+
+    // ---- conv, head mix, softmax statistics
+    const int tid = threadIdx.x - ROLE_THREADS;
     load_mix(W_sm, a.W1, H, a.w_dtype);
-    for (int i = threadIdx.x; i < (H + 1) / 2 * a.cq * ckp; i += THREADS) {
+    for (int i = tid; i < (H + 1) / 2 * a.cq * ckp; i += ROLE_THREADS) {
         const int j = i % ckp, row = i / ckp, tap = row % a.cq, h = row / a.cq * 2;
         const long at = ((long)h * a.cq + tap) * a.ck + j;
         t_sm[i] = make_float2(j < a.ck ? load_weight(a.w1, at, a.w_dtype) * a.scale : 0.0f,
                               j < a.ck && h + 1 < H ? load_weight(a.w1, at + a.cq * a.ck, a.w_dtype) * a.scale : 0.0f);
     }
-    // positions that hold no score yet are read with taps of zero: they have to be finite
-    for (int i = threadIdx.x; i < (a.kv_together * group + 1) / 2 * R * ring.row / 4; i += THREADS) reinterpret_cast<float4*>(s_sm)[i] = make_float4(0, 0, 0, 0);
-    __syncthreads();
-    const long n = before[a.B], workers = n < a.workers ? n : a.workers, me = blockIdx.x;
-    if (me >= workers) return;
-    const long end = run_begin(me + 1, n, workers);
-    const T* pool = static_cast<const T*>(c.k);
-    const T* queries = static_cast<const T*>(c.q_hist);
-    const bool whole = a.kv_together == c.kv_heads;              // all heads at once: what tiles share stays in the ring
     const int quads = tile / 4, oquads = round4(H) / 4;
-
-    for (long x = run_begin(me, n, workers); x < end;) {
-        const int b = find_line(before, a.B, x), len = lens[b], slot = c.slot(b);
-        const int ta = (int)(x - before[b]), tb = (int)(end - before[b] < before[b + 1] - before[b] ? end - before[b] : before[b + 1] - before[b]);
-        for (int i = threadIdx.x; i < a.cq2 * H; i += THREADS) ml[i] = make_float2(-INFINITY, 0.0f);
-        if (threadIdx.x < DECODE_MAX_ROWS) {
-            const int pos = len - R + threadIdx.x;
-            q_at[threadIdx.x] = threadIdx.x < R && pos >= 0 ? ((long)slot * c.ring + pos % c.ring) * H * c.D : -1;
-        }
-        __syncthreads();
-        for (int tl = ta; tl < tb; ++tl) {
-            const int k0 = tl << a.shift;
-            if (tl + 1 < tb) prefetch_tile(c, pool, slot, k0 + tile + hr, tile, len);
-            for (int hk0 = 0; hk0 < c.kv_heads; hk0 += a.kv_together) {
-                const int nk = c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together;
-                // scores of the keys that the ring does not hold yet, one (kv head, 16 keys) a warp and step
-                const int first = whole && tl > ta ? k0 + hr : k0 - hl, units = (k0 + tile + hr - first) / KEYS, tasks = nk * units;
-                K keys;
-                uint4 q[HALF ? NT : 1][HALF ? K::CH : 1];
-                auto fetch = [&](int hk, int key) {
-                    keys.load(pool, key >= 0 && key < len ? c.at(slot, hk0 + hk, key) : -1L, len - key < KEYS ? len - key : KEYS, c.D, lane);
-                };
-                int task = warp * tasks / WARPS;
-                const int last = (warp + 1) * tasks / WARPS;
-                int hk = task / units, u = task - hk * units, q_head = -1;
-                if (task < last) fetch(hk, first + u * KEYS);
-                while (task < last) {
-                    const int key = first + u * KEYS, hk_now = hk;
-                    ++task;
-                    if (++u == units) { u = 0; ++hk; }
-                    int at = (key + shift + ring.keys) % ring.keys + g;              // ring position of key `g` of the unit
-                    const bool full = key + KEYS - 1 <= len - R;                     // every row sees every key
-                    for (int gq = 0; gq < group; ++gq) {
-                        const int h = hk_now * group + gq;
-                        const T* qh = queries + (long)(hk0 * group + h) * c.D;
-                        float acc[NT][4];
-                        if constexpr (HALF) {
-                            if (q_head != h) {
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    const long row = q_at[8 * nt + g];
-#pragma unroll
-                                    for (int ch = 0; ch < K::CH; ++ch) {
-                                        const int e = (ch * 4 + t4) * K::EPL;
-                                        q[nt][ch] = row >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + row + e) : make_uint4(0, 0, 0, 0);
-                                    }
-                                }
-                                q_head = h;
-                            }
-                            keys.template score<NT>(acc, lane, [&](int nt, int ch) { return q[nt][ch]; });
-                        } else {
-                            keys.template score<NT>(acc, lane, [&](int row, int ch) {
-                                const long r = q_at[row];
-                                const int e = (ch * 4 + t4) * K::EPL;
-                                return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
-                            });
-                        }
-                        if (gq == group - 1 && task < last) fetch(hk, first + u * KEYS);
-                        float* s = s_sm + (long)(h >> 1) * R * ring.row + (h & 1);
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            int pos = at + 8 * y;
-                            if (pos >= ring.keys) pos -= ring.keys;
-                            const int place = (pos & 2 ? ring.half : 0) + (pos >> 2) * 4 + (pos & 1) * 2, kk = key + g + 8 * y;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                                for (int z = 0; z < 2; ++z) {
-                                    const int row = 8 * nt + 2 * t4 + z;
-                                    if (row < R) s[row * ring.row + place] = full || kk <= len - R + row ? acc[nt][2 * y + z] : 0.0f;
-                                }
-                            }
-                        }
-                    }
-                }
-                __syncthreads();
+    int stage = 0, stages = 0;                                   // of the whole run: what is not waited for at its end
+    for (long x = begin; x < end;) {
+        const Span s = span_at(c, before, lens, a.B, x, end);
+        stages += (s.k1 - s.k0 + tile - 1) / tile * ((c.kv_heads + a.kv_together - 1) / a.kv_together);
+        x = (long)before[s.b] + s.k1 / KEYS;
+    }
+    int turn = 0;
+    for (long x = begin; x < end;) {
+        const Span s = span_at(c, before, lens, a.B, x, end);
+        turn = ring_turn(ring, whole, turn, s.k0 - hl);
+        for (int i = tid; i < a.cq2 * H * quads; i += ROLE_THREADS) ml[i] = make_float2(-INFINITY, 0.0f);
+        const int limit = s.k1 < s.len ? s.k1 : s.len;           // keys from here on are another run's
+        for (int k0 = s.k0; k0 < s.k1; k0 += tile) {
+            for (int hk0 = 0; hk0 < c.kv_heads; hk0 += a.kv_together, ++stage) {
+                barrier_sync(BAR_FULL + (stage & 1), THREADS);
                 // conv: (two heads, row, four keys) a thread
-                const int heads = nk * group, pairs = (heads + 1) / 2;
-                int q0 = k0 - left + shift;                                          // a multiple of 4
-                q0 = ((q0 + ring.keys) % ring.keys) >> 2;
-                for (int i = threadIdx.x; i < pairs * a.cq2 << (a.shift - 2); i += THREADS) {
+                const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group, pairs = (heads + 1) / 2;
+                const int q0 = ((k0 - left + turn + shift) % ring.keys) >> 2;
+                for (int i = tid; i < pairs * a.cq2 << (a.shift - 2); i += ROLE_THREADS) {
                     const int quad = i & (quads - 1), rest = i >> (a.shift - 2), r = rest / pairs, pair = rest - r * pairs;
                     int q1 = q0 + quad;
                     if (q1 >= ring.keys / 4) q1 -= ring.keys / 4;
                     float2 z[4];
                     z[0] = z[1] = z[2] = z[3] = make_float2(0.0f, 0.0f);
-                    const float* srow = s_sm + ((long)pair * R + r) * ring.row;
-                    const float4* w = reinterpret_cast<const float4*>(t_sm + (long)(hk0 * group / 2 + pair) * a.cq * ckp);
+                    const float* srow = s_sm + (stage & 1) * s_other + (pair * R + r) * ring.row;
+                    const float4* w = reinterpret_cast<const float4*>(t_sm + (hk0 * group / 2 + pair) * a.cq * ckp);
                     for (int tap = 0; tap < a.cq; ++tap, srow += ring.row) {
                         const float4 *e4 = reinterpret_cast<const float4*>(srow), *o4 = reinterpret_cast<const float4*>(srow + ring.half);
                         int at = q1;
@@ -275,67 +408,72 @@ __global__ void __launch_bounds__(THREADS, scores_blocks((int)sizeof(T), DMAX, N
                         for (int j = 0; j < ckp / 4; ++j, w += 2) {
                             at = at + 1 == ring.keys / 4 ? 0 : at + 1;
                             const float4 e1 = e4[at], o1 = o4[at], wa = w[0], wb = w[1];
-                            const float2 s[7] = {make_float2(e.x, e.y), make_float2(e.z, e.w), make_float2(o.x, o.y), make_float2(o.z, o.w),
+                            const float2 v[7] = {make_float2(e.x, e.y), make_float2(e.z, e.w), make_float2(o.x, o.y), make_float2(o.z, o.w),
                                                  make_float2(e1.x, e1.y), make_float2(e1.z, e1.w), make_float2(o1.x, o1.y)};
                             const float2 ws[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
 #pragma unroll
                             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) z[k] = __ffma2_rn(ws[t], s[k + t], z[k]);
+                                for (int k = 0; k < 4; ++k) z[k] = __ffma2_rn(ws[t], v[k + t], z[k]);
                             e = e1; o = o1;
                         }
                     }
-                    float* to = c_sm + (((long)r * H + hk0 * group + 2 * pair) << a.shift) + 4 * quad;
+                    float* to = c_sm + ((r * H + hk0 * group + 2 * pair) << a.shift) + 4 * quad;
                     *reinterpret_cast<float4*>(to) = make_float4(z[0].x, z[1].x, z[2].x, z[3].x);
                     if (2 * pair + 1 < heads) *reinterpret_cast<float4*>(to + tile) = make_float4(z[0].y, z[1].y, z[2].y, z[3].y);
                 }
-                __syncthreads();
+                if (stage + 2 < stages) barrier_arrive(BAR_EMPTY + (stage & 1), THREADS);
             }
-            // head mix and softmax statistics: (row, four heads, four keys) a thread; the threads of a row and four heads are neighbours
-            for (int i0 = warp * 32; i0 < a.cq2 * oquads << (a.shift - 2); i0 += THREADS) {
-                const int i = i0 + lane, kq = (i & (quads - 1)) * 4, rest = i >> (a.shift - 2), r0 = rest / oquads, o0 = (rest - r0 * oquads) * 4;
-                const bool on = r0 < a.cq2;
-                const int r = on ? r0 : 0;
+            barrier_sync(BAR_MATH, ROLE_THREADS);
+            // head mix and softmax statistics: (row, four heads, four keys) a thread
+            for (int i = tid; i < a.cq2 * oquads << (a.shift - 2); i += ROLE_THREADS) {
+                const int kq = (i & (quads - 1)) * 4, rest = i >> (a.shift - 2), r = rest / oquads, o0 = (rest - r * oquads) * 4;
+                if (k0 + kq >= limit) continue;
                 float z[4][4];
-                mix_heads(z, W_sm + o0, c_sm + (((long)r * H) << a.shift) + kq, H, tile);
-                const int seen = len - a.cq2 + r - k0 - kq;                          // of the four keys those up to this one are seen by the row
+                mix_heads(z, W_sm + o0, c_sm + ((r * H) << a.shift) + kq, H, tile);
+                const int seen = s.len - a.cq2 + r - k0 - kq;                        // of the four keys those up to this one are seen by the row
 #pragma unroll
                 for (int o = 0; o < 4; ++o) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (k > seen) z[o][k] = -INFINITY;
                     const int row = r * H + o0 + o;
-                    const bool put = on && o0 + o < H;
-                    const float2 old = put ? ml[row] : make_float2(0.0f, 0.0f);
-                    float top = fmaxf(fmaxf(z[o][0], z[o][1]), fmaxf(z[o][2], z[o][3]));
-                    for (int s = 1; s < quads; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                    top = fmaxf(top, old.x);
-                    // while a row has seen nothing its maximum is -inf and its sum 0
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    float sum = 0.0f;
+                    if (o0 + o < H) {
+                        // maximum and sum of this thread's own keys of the run
+                        const float2 old = ml[row * quads + kq / 4];
+                        const float top = fmaxf(fmaxf(fmaxf(z[o][0], z[o][1]), fmaxf(z[o][2], z[o][3])), old.x);
+                        // while nothing has been seen the maximum is -inf and the sum 0
+                        const float ref = top == -INFINITY ? 0.0f : top;
+                        float sum = old.y * fast_exp2(old.x - ref);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) sum += fast_exp2(z[o][k] - ref);
-                    for (int s = 1; s < quads; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-                    if (put) {
-                        *reinterpret_cast<float4*>(a.logits + ((long)b * a.cq2 * H + row) * a.pitch + k0 + kq) = make_float4(z[o][0], z[o][1], z[o][2], z[o][3]);
-                        if (kq == 0) ml[row] = make_float2(top, fmaf(old.y, fast_exp2(old.x - ref), sum));
+                        for (int k = 0; k < 4; ++k) sum += fast_exp2(z[o][k] - ref);
+                        ml[row * quads + kq / 4] = make_float2(top, sum);
+                        *reinterpret_cast<float4*>(a.logits + ((long)s.b * a.cq2 * H + row) * a.pitch + k0 + kq) = make_float4(z[o][0], z[o][1], z[o][2], z[o][3]);
                     }
                 }
             }
-            // the next tile's scores go to places of the ring that this tile's conv, two barriers back, was the last to read
+            barrier_sync(BAR_MATH, ROLE_THREADS);                // the next tile's conv writes where this mix reads
         }
-        __syncthreads();
-        const long part = me + b;
-        for (int i = threadIdx.x; i < a.cq2 * H; i += THREADS) a.part_ml[part * a.cq2 * H + i] = ml[i];
-        __syncthreads();
-        x = (long)before[b] + tb;
+        for (int i = tid; i < a.cq2 * H; i += ROLE_THREADS) {
+            float top = -INFINITY, sum = 0.0f;
+            for (int k = 0; k < quads; ++k) top = fmaxf(top, ml[i * quads + (k + i) % quads].x);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            for (int k = 0; k < quads; ++k) {
+                const float2 v = ml[i * quads + (k + i) % quads];
+                sum = fmaf(v.y, fast_exp2(v.x - ref), sum);
+            }
+            a.part_ml[(me + s.b) * a.cq2 * H + i] = make_float2(top, sum);
+        }
+        barrier_sync(BAR_MATH, ROLE_THREADS);
+        turn += s.k0 + (s.k1 - s.k0 + tile - 1) / tile * tile + hr;                  // the place behind the span's last tile
+        x = (long)before[s.b] + s.k1 / KEYS;
     }
 }
 
-// Tasks of (GT query heads, share of a tile's keys) are dealt to warps; where there are fewer heads than warps, `copies` warps share
-// one and each keeps an output of its own.
+// Tasks of (GT query heads, share of a tile's keys) belong to one warp each; where heads do not divide evenly among the warps, `copies`
+// warps share one and each keeps an output of its own.
 template <typename T, int DMAX, int GT>
-__global__ void __launch_bounds__(THREADS, sizeof(T) * DMAX > 256 ? 1 : 2) mta_decode_values_kernel(PagedCache c, MtaArgs a, int copies) {
+__global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCache c, MtaArgs a, int copies) {
     constexpr bool HALF = sizeof(T) == 2;
     using V = std::conditional_t<HALF, ValueTile<T, DMAX>, ValueTileF32<DMAX>>;
     using P = Pieces<GT>;
@@ -346,158 +484,178 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) * DMAX > 256 ? 1 : 2) mta_d
     const ValueSmem m = value_smem(a.B, H, c.D, tile, a.cq2, a.ck2, copies);
     float *p_sm = reinterpret_cast<float*>(smem + m.p), *y_sm = reinterpret_cast<float*>(smem + m.y), *by = reinterpret_cast<float*>(smem + m.by);
     float *W_sm = reinterpret_cast<float*>(smem + m.W), *t_sm = reinterpret_cast<float*>(smem + m.taps), *o_sm = reinterpret_cast<float*>(smem + m.o);
-    T* a_sm = reinterpret_cast<T*>(smem + m.a);                  // [head][piece][key], float32: [head][key]
-    float2* ml = reinterpret_cast<float2*>(smem + m.ml);
+    T* a_sm = reinterpret_cast<T*>(smem + m.a);                  // by the stage's parity: [head][piece][key], float32: [head][key]
+    const int a_other = (int)(m.a_one / sizeof(T));
+    float *top_sm = reinterpret_cast<float*>(smem + m.ml), *r_sm = reinterpret_cast<float*>(smem + m.run_taps);
     int *before = reinterpret_cast<int*>(smem + m.before), *lens = before + a.B + 1;
 
-    // nothing up to pdl_wait() is written by the kernel before
-    count_tiles(c, a.B, a.shift, before, lens);
-    load_mix(W_sm, a.W2, H, a.w_dtype);
-    for (int i = threadIdx.x; i < H * a.cq2 * ckp; i += THREADS) {
-        const int j = i % ckp, row = i / ckp;
-        t_sm[i] = j < a.ck2 ? load_weight(a.w2, (long)row * a.ck2 + j, a.w_dtype) : 0.0f;
-    }
+    // The lengths, the tables, the values and the weights are not written by the kernel before.
+    count_tiles(c, a.B, 4, before, lens);
     __syncthreads();
-    const T* pool = static_cast<const T*>(c.v);
     const long n = before[a.B], workers = n < a.workers ? n : a.workers, me = blockIdx.x;
-    const long begin = run_begin(me, n, workers > 0 ? workers : 1), end = run_begin(me + 1, n, workers > 0 ? workers : 1);
-    if (me < workers) {
-        const int b = find_line(before, a.B, begin);
-        prefetch_tile(c, pool, c.slot(b), (int)(begin - before[b]) << a.shift, tile, lens[b]);
-    }
-    if constexpr (std::is_same_v<T, __half>) {
-        // Probabilities are at most 1, so a weight of head o is at most A = sum_h |W2[o,h]| sum |w2[h]|.  Times 2^14 over the power of two
-        // below A it stays under 2^15, and its pieces are out of fp16's subnormal numbers down to 2^-28 A.
-        for (int h = threadIdx.x; h < H; h += THREADS) {
-            float s = 0.0f;
-            for (int i = 0; i < a.cq2 * ckp; ++i) s += fabsf(t_sm[h * a.cq2 * ckp + i]);
-            y_sm[h] = s;
-        }
-        __syncthreads();
-        for (int o = threadIdx.x; o < H; o += THREADS) {
-            float s = 0.0f;
-            for (int h = 0; h < H; ++h) s = fmaf(fabsf(W_sm[h * round4(H) + o]), y_sm[h], s);
-            by[o] = s > 1e-30f && s < 1e30f ? exp2f((float)(14 - ilogbf(s))) : 1.0f;
-        }
-        __syncthreads();
-    }
-    pdl_wait();
     if (me >= workers) return;
+    const long begin = run_begin(me, n, workers), end = run_begin(me + 1, n, workers);
 
-    for (long x = begin; x < end;) {
-        const int b = find_line(before, a.B, x), len = lens[b], slot = c.slot(b), tiles = before[b + 1] - before[b];
-        const int ta = (int)(x - before[b]), tb = (int)(end - before[b] < tiles ? end - before[b] : tiles);
-        const long w0 = run_owner(before[b], n, workers), w1 = run_owner((long)before[b] + tiles - 1, n, workers);
-        // maximum and one over the sum of every (row, head), from all runs of the sequence: eight lanes each
-        for (int i0 = threadIdx.x / 8; i0 < (a.cq2 * H + 31) / 32 * 32; i0 += THREADS / 8) {
-            const int i = i0 < a.cq2 * H ? i0 : a.cq2 * H - 1;
-            float top = -INFINITY, sum = 0.0f;
-            for (long w = w0 + threadIdx.x % 8; w <= w1; w += 8) {
-                const float2 v = a.part_ml[(w + b) * a.cq2 * H + i];
-                const float t = fmaxf(top, v.x), ref = t == -INFINITY ? 0.0f : t;
-                sum = fmaf(sum, fast_exp2(top - ref), v.y * fast_exp2(v.x - ref));
-                top = t;
+    if (warp >= ROLE_WARPS) {
+        // ---- product with the values.  A stage is a tile; the loads run ahead of the arithmetic as in the scores kernel.
+        const int tid = threadIdx.x - ROLE_THREADS, me_warp = warp - ROLE_WARPS, tasks = H / GT * copies;
+        const T* pool = static_cast<const T*>(c.v);
+        struct Cursor {
+            Span s;
+            long at;
+            int k0, units, task, unit, last, taken, stage;
+            Pages next;
+            bool done;
+        } cur = {};
+        auto share = [&] {                                       // the units of this stage that the task's copy has
+            const int copy = cur.task % copies, all = tile / KEYS;
+            cur.unit = copy * all / copies;
+            cur.last = (copy + 1) * all / copies < cur.units ? (copy + 1) * all / copies : cur.units;
+        };
+        // L2 is asked for the tile at k0, a (kv head, unit) per thread of this half; `at` is the place of the lane's unit.
+        auto ask_l2 = [&](int k0, long at) {
+            const int units = ((k0 + tile < cur.s.k1 ? k0 + tile : cur.s.k1) - k0) / KEYS, all = c.kv_heads * units;
+            for (int t = me_warp * 32; t < all; t += ROLE_THREADS) {
+                const int mine = t + lane < all ? t + lane : all - 1, hk = mine / units, unit = mine - hk * units;
+                const long base = __shfl_sync(0xffffffffu, at, unit);
+                const int live = cur.s.len - (k0 + unit * KEYS);
+                if (t + lane < all && base >= 0) prefetch_l2(pool + base + ((long)hk << c.page_shift) * c.D, (uint32_t)((live < KEYS ? live : KEYS) * c.D * sizeof(T)));
             }
-#pragma unroll
-            for (int s = 1; s < 8; s <<= 1) {
-                const float v = __shfl_xor_sync(0xffffffffu, top, s), l = __shfl_xor_sync(0xffffffffu, sum, s);
-                const float t = fmaxf(top, v), ref = t == -INFINITY ? 0.0f : t;
-                sum = sum * fast_exp2(top - ref) + l * fast_exp2(v - ref);
-                top = t;
+        };
+        auto enter_stage = [&] {
+            cur.units = ((cur.k0 + tile < cur.s.k1 ? cur.k0 + tile : cur.s.k1) - cur.k0) / KEYS;
+            const int key = cur.k0 + lane * KEYS;
+            const bool on = lane < cur.units && key < cur.s.len;
+            if (cur.k0 == cur.s.k0) cur.next.look_up(c, cur.s.slot, key, on);
+            cur.at = cur.next.at(c, key, on);
+            if (cur.k0 == cur.s.k0) ask_l2(cur.k0, cur.at);
+            const bool ahead = lane < tile / KEYS && key + tile < cur.s.len;
+            cur.next.look_up(c, cur.s.slot, key + tile, ahead);
+            cur.taken = 0;
+            cur.task = me_warp;
+            share();
+        };
+        auto enter_span = [&](long x) {
+            cur.s = span_at(c, before, lens, a.B, x, end);
+            cur.k0 = cur.s.k0;
+        };
+        enter_span(begin);
+        enter_stage();
+        V values;
+        int t_task = 0, t_unit = 0;                              // whose values are on their way
+        bool t_first = false, t_final = false;                   // of its task and stage
+        auto fetch = [&]() -> bool {
+            while (!cur.done && (cur.task >= tasks || cur.unit >= cur.last)) {
+                if (cur.task < tasks) {
+                    cur.task += ROLE_WARPS;
+                    if (cur.task < tasks) share();
+                    continue;
+                }
+                ++cur.stage;
+                cur.k0 += tile;
+                if (cur.k0 >= cur.s.k1) {
+                    const long x = (long)before[cur.s.b] + cur.s.k1 / KEYS;
+                    if (x >= end) { cur.done = true; break; }
+                    enter_span(x);
+                }
+                enter_stage();
             }
-            // a row before the first token has no keys: its probabilities are zero
-            if (threadIdx.x % 8 == 0 && i0 < a.cq2 * H) ml[i] = len - a.cq2 + i / H < 0 ? make_float2(0.0f, 0.0f) : make_float2(top, 1.0f / sum);
+            if (cur.done) return false;
+            const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
+            const int copy = cur.task % copies, hk = cur.task / copies * GT / group;
+            t_task = cur.task; t_unit = cur.unit;
+            t_first = cur.unit == copy * (tile / KEYS) / copies;
+            values.load(pool, base < 0 ? base : base + ((long)hk << c.page_shift) * c.D, cur.s.len - (cur.k0 + cur.unit * KEYS), c.D, lane);
+            t_final = ++cur.unit == cur.last;
+            if (++cur.taken == 2 && cur.k0 + tile < cur.s.k1) {
+                const int ahead = cur.k0 + tile + lane * KEYS;
+                ask_l2(cur.k0 + tile, cur.next.at(c, ahead, lane < tile / KEYS && ahead < cur.s.len));
+            }
+            return true;
+        };
+        int stage = 0, stages = 0;
+        for (long x = begin; x < end;) {
+            const Span s = span_at(c, before, lens, a.B, x, end);
+            stages += (s.k1 - s.k0 + tile - 1) / tile;
+            x = (long)before[s.b] + s.k1 / KEYS;
         }
-        for (int i = threadIdx.x; i < copies * H * c.D; i += THREADS) o_sm[i] = 0.0f;
-        __syncthreads();
-        for (int tl = ta; tl < tb; ++tl) {
-            const int k0 = tl << a.shift;
-            if (tl + 1 < tb) prefetch_tile(c, pool, slot, k0 + tile, tile, len);
-            for (int row = warp; row < a.cq2 * H; row += WARPS) {
-                const float2 s = ml[row];
-                const float* from = a.logits + ((long)b * a.cq2 * H + row) * a.pitch;
-                for (int col = lane; col < pp; col += 32) {
-                    const int key = k0 - left + col;
-                    p_sm[row * pp + col] = key >= 0 && key < len && col < tile + a.ck2 - 1 ? fast_exp2(from[key] - s.x) * s.y : 0.0f;
+        for (int i = tid; i < copies * H * c.D; i += ROLE_THREADS) o_sm[i] = 0.0f;
+        constexpr int CH = HALF ? DMAX / 64 : 1;
+        float acc[HALF ? CH : GT][4][4];                         // mma accumulators; float32: [head][0][element]
+        // The outputs of a span, once all of this half are done with it.
+        auto put_out = [&](int b) {
+            barrier_sync(BAR_MEMORY, ROLE_THREADS);
+            const long u0 = before[b], u1 = before[b + 1];
+            const bool only = run_owner(u0, n, workers) == run_owner(u1 - 1, n, workers);
+            for (int i = tid; i < H * c.D; i += ROLE_THREADS) {
+                float v = 0.0f;
+                for (int y = 0; y < copies; ++y) {
+                    v += o_sm[y * H * c.D + i];
+                    o_sm[y * H * c.D + i] = 0.0f;
                 }
+                if (only) static_cast<T*>(a.out)[(long)b * H * c.D + i] = from_f32<T>(v);      // the only run of the sequence
+                else a.part_o[(me + b) * H * c.D + i] = v;
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < H << (a.shift - 2); i += THREADS) {
-                const int quad = i & (quads - 1), h = i >> (a.shift - 2);
-                float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int tap = 0; tap < a.cq2; ++tap) conv_row(z, p_sm + (tap * H + h) * pp + 4 * quad, t_sm + (h * a.cq2 + tap) * ckp, ckp);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (k0 + 4 * quad + e >= len) z[e] = 0.0f;
-                *reinterpret_cast<float4*>(y_sm + (h << a.shift) + 4 * quad) = make_float4(z[0], z[1], z[2], z[3]);
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < oquads << (a.shift - 2); i += THREADS) {
-                const int kq = (i & (quads - 1)) * 4, o0 = (i >> (a.shift - 2)) * 4;
-                float z[4][4];
-                mix_heads(z, W_sm + o0, y_sm + kq, H, tile);
-#pragma unroll
-                for (int o = 0; o < 4; ++o) {
-                    if (o0 + o >= H) break;
-                    if constexpr (HALF) {
-                        float f[4][P::PIECES];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) split_pieces<T>(std::is_same_v<T, __half> ? z[o][k] * by[o0 + o] : z[o][k], f[k]);
-#pragma unroll
-                        for (int piece = 0; piece < P::PIECES; ++piece)
-                            *reinterpret_cast<uint2*>(a_sm + ((o0 + o) * P::PIECES + piece) * ap + kq) =
-                                make_uint2(pack2<T>(f[0][piece], f[1][piece]), pack2<T>(f[2][piece], f[3][piece]));
-                    } else {
-                        *reinterpret_cast<float4*>(a_sm + ((o0 + o) << a.shift) + kq) = make_float4(z[o][0], z[o][1], z[o][2], z[o][3]);
+            barrier_sync(BAR_MEMORY, ROLE_THREADS);
+        };
+        // Every warp of this half passes every stage, with or without a task in it, and the ends of spans between them, so that all meet
+        // the same barriers in the same order.
+        long span_x = begin;
+        Span span = span_at(c, before, lens, a.B, begin, end);
+        int span_end = (span.k1 - span.k0 + tile - 1) / tile;    // the stage behind the span's last
+        auto pass_stages = [&](int to) {
+            while (stage < to) {
+                if (stage + 2 < stages) barrier_arrive(BAR_EMPTY + (stage & 1), THREADS);
+                if (++stage == span_end) {
+                    put_out(span.b);
+                    span_x = (long)before[span.b] + span.k1 / KEYS;
+                    if (span_x < end) {
+                        span = span_at(c, before, lens, a.B, span_x, end);
+                        span_end += (span.k1 - span.k0 + tile - 1) / tile;
                     }
                 }
+                if (stage < stages) barrier_sync(BAR_FULL + (stage & 1), THREADS);
             }
-            __syncthreads();
-            // product with the values
-            const int units = tile / KEYS, tasks = H / GT * copies;
-            for (int task = warp; task < tasks; task += WARPS) {
-                const int copy = task % copies, h0 = task / copies * GT, hk = h0 / group;
-                int u = copy * units / copies;
-                const int live_units = (len - k0 + KEYS - 1) / KEYS, ub = (copy + 1) * units / copies < live_units ? (copy + 1) * units / copies : live_units;
-                if (u >= ub) continue;
-                V values;
-                auto fetch = [&](int unit) {
-                    const int key = k0 + unit * KEYS;
-                    values.load(pool, c.at(slot, hk, key), len - key < KEYS ? len - key : KEYS, c.D, lane);
-                };
-                fetch(u);
-                if constexpr (HALF) {
-                    float acc[V::CHUNKS][4][4];
+        };
+        barrier_sync(BAR_MEMORY, ROLE_THREADS);                  // the outputs are zero
+        bool started = false;
+        for (bool more = fetch(); more;) {
+            // the cursor still stands where this task's values were fetched
+            if (!started) barrier_sync(BAR_FULL, THREADS);       // the first stage
+            started = true;
+            pass_stages(cur.stage);
+            const int unit = t_unit, copy = t_task % copies, h0 = t_task / copies * GT;
+            const bool first = t_first, final = t_final;
+            const T* weights = a_sm + (stage & 1) * a_other;
+            if (first) {
 #pragma unroll
-                    for (int i = 0; i < V::CHUNKS; ++i)
+                for (int i = 0; i < (HALF ? CH : GT); ++i)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
-                    const int y = g / P::STRIDE, piece = g % P::STRIDE;
-                    const bool on = y < GT && piece < P::PIECES;
-                    const uint32_t* col = reinterpret_cast<const uint32_t*>(a_sm + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4;
-                    for (; u < ub; ++u) {
-                        values.multiply(acc, on ? col[u * 8] : 0u, on ? col[u * 8 + 4] : 0u);
-                        if (u + 1 < ub) fetch(u + 1);
-                    }
+                    for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
+            }
+            if constexpr (HALF) {
+                const int y = g / P::STRIDE, piece = g % P::STRIDE;
+                const bool on = y < GT && piece < P::PIECES;
+                const uint32_t* col = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4 + unit * 8;
+                values.multiply(acc, on ? col[0] : 0u, on ? col[4] : 0u);
+                more = fetch();
+                if (final) {
                     // sum over the pieces; a head's columns are those of one lane (four heads) or of two, which then halve the elements
-                    constexpr int CH = V::CHUNKS;
-                    float f[CH][8];
-#pragma unroll
-                    for (int i = 0; i < CH; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { f[i][j] = acc[i][j][0] + acc[i][j][1]; f[i][j + 4] = acc[i][j][2] + acc[i][j][3]; }
                     const int head = h0 + t4 * 2 / P::STRIDE;
                     const bool mine = t4 * 2 / P::STRIDE < GT;
-                    float* to = o_sm + ((long)copy * H + (mine ? head : 0)) * c.D;
+                    float* to = o_sm + (copy * H + (mine ? head : 0)) * c.D;
                     const float back = std::is_same_v<T, __half> && mine ? 1.0f / by[head] : 1.0f;
 #pragma unroll
                     for (int i = 0; i < CH; ++i) {
+                        float f[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { f[j] = acc[i][j][0] + acc[i][j][1]; f[j + 4] = acc[i][j][2] + acc[i][j][3]; }
                         const int e0 = i * 64 + g * 8;
                         if constexpr (P::STRIDE == 4) {
                             float h[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float give = t4 & 1 ? f[i][e] : f[i][e + 4], keep = t4 & 1 ? f[i][e + 4] : f[i][e];
+                                const float give = t4 & 1 ? f[e] : f[e + 4], keep = t4 & 1 ? f[e + 4] : f[e];
                                 h[e] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
                             }
                             if (mine && e0 < c.D) {
@@ -511,56 +669,165 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) * DMAX > 256 ? 1 : 2) mta_d
                             for (int e = 0; e < 8; e += 4) {
                                 float4* at = reinterpret_cast<float4*>(to + e0 + e);
                                 float4 v = *at;
-                                v.x = fmaf(f[i][e], back, v.x); v.y = fmaf(f[i][e + 1], back, v.y); v.z = fmaf(f[i][e + 2], back, v.z); v.w = fmaf(f[i][e + 3], back, v.w);
+                                v.x = fmaf(f[e], back, v.x); v.y = fmaf(f[e + 1], back, v.y); v.z = fmaf(f[e + 2], back, v.z); v.w = fmaf(f[e + 3], back, v.w);
                                 *at = v;
                             }
                         }
                     }
-                } else {
-                    float o[GT][4];
+                }
+            } else {
 #pragma unroll
-                    for (int y = 0; y < GT; ++y) o[y][0] = o[y][1] = o[y][2] = o[y][3] = 0.0f;
-                    for (; u < ub; ++u) {
+                for (int i = 0; i < V::STEPS; ++i) {
+                    float f[4];
+                    unpack16<float>(values.r[i], f);
 #pragma unroll
-                        for (int i = 0; i < V::STEPS; ++i) {
-                            float f[4];
-                            unpack16<float>(values.r[i], f);
+                    for (int y = 0; y < GT; ++y) {
+                        const float p = weights[((h0 + y) << a.shift) + unit * KEYS + i * V::SUBS + lane / V::ROWLANES];
 #pragma unroll
-                            for (int y = 0; y < GT; ++y) {
-                                const float p = a_sm[((h0 + y) << a.shift) + u * KEYS + i * V::SUBS + lane / V::ROWLANES];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[y][e] = fmaf(p, f[e], o[y][e]);
-                            }
-                        }
-                        if (u + 1 < ub) fetch(u + 1);
+                        for (int e = 0; e < 4; ++e) acc[y][0][e] = fmaf(p, f[e], acc[y][0][e]);
                     }
+                }
+                more = fetch();
+                if (final) {
                     const int e0 = (lane % V::ROWLANES) * 4;
 #pragma unroll
                     for (int y = 0; y < GT; ++y) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
-                            for (int s = V::ROWLANES; s < 32; s <<= 1) o[y][e] += __shfl_xor_sync(0xffffffffu, o[y][e], s);
+                            for (int s = V::ROWLANES; s < 32; s <<= 1) acc[y][0][e] += __shfl_xor_sync(0xffffffffu, acc[y][0][e], s);
                         if (lane < V::ROWLANES && e0 < c.D) {
-                            float4* at = reinterpret_cast<float4*>(o_sm + ((long)copy * H + h0 + y) * c.D + e0);
+                            float4* at = reinterpret_cast<float4*>(o_sm + (copy * H + h0 + y) * c.D + e0);
                             float4 v = *at;
-                            v.x += o[y][0]; v.y += o[y][1]; v.z += o[y][2]; v.w += o[y][3];
+                            v.x += acc[y][0][0]; v.y += acc[y][0][1]; v.z += acc[y][0][2]; v.w += acc[y][0][3];
                             *at = v;
                         }
                     }
                 }
             }
-            // the next writes of p come after every thread's conv, those of y and of the weights behind the next barriers
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < H * c.D; i += THREADS) {
-            float v = 0.0f;
-            for (int y = 0; y < copies; ++y) v += o_sm[(long)y * H * c.D + i];
-            if (w0 == w1) static_cast<T*>(a.out)[(long)b * H * c.D + i] = from_f32<T>(v);      // the only run of the sequence
-            else a.part_o[(me + b) * H * c.D + i] = v;
+        if (!started) barrier_sync(BAR_FULL, THREADS);           // no task at all
+        pass_stages(stages);
+        return;
+    }
+
+    // ---- probabilities, conv, head mix: the weights of the values
+    const int tid = threadIdx.x;
+    load_mix(W_sm, a.W2, H, a.w_dtype);
+    for (int i = tid; i < H * a.cq2 * ckp; i += ROLE_THREADS) {
+        const int j = i % ckp, row = i / ckp;
+        t_sm[i] = j < a.ck2 ? load_weight(a.w2, (long)row * a.ck2 + j, a.w_dtype) : 0.0f;
+    }
+    barrier_sync(BAR_MATH, ROLE_THREADS);
+    if constexpr (std::is_same_v<T, __half>) {
+        // Probabilities are at most 1, so a weight of head o is at most A = sum_h |W2[o,h]| sum |w2[h]|.  Times 2^14 over the power of two
+        // below A it stays under 2^15, and its pieces are out of fp16's subnormal numbers down to 2^-28 A.
+        for (int h = tid; h < H; h += ROLE_THREADS) {
+            float s = 0.0f;
+            for (int i = 0; i < a.cq2 * ckp; ++i) s += fabsf(t_sm[h * a.cq2 * ckp + i]);
+            y_sm[h] = s;
         }
-        __syncthreads();
-        x = (long)before[b] + tb;
+        barrier_sync(BAR_MATH, ROLE_THREADS);
+        for (int o = tid; o < H; o += ROLE_THREADS) {
+            float s = 0.0f;
+            for (int h = 0; h < H; ++h) s = fmaf(fabsf(W_sm[h * round4(H) + o]), y_sm[h], s);
+            by[o] = s > 1e-30f && s < 1e30f ? exp2f((float)(14 - ilogbf(s))) : 1.0f;
+        }
+        barrier_sync(BAR_MATH, ROLE_THREADS);
+    }
+    pdl_wait();
+    int stage = 0;
+    for (long x = begin; x < end;) {
+        const Span s = span_at(c, before, lens, a.B, x, end);
+        const long w0 = run_owner(before[s.b], n, workers), w1 = run_owner((long)before[s.b + 1] - 1, n, workers);
+        // maximum and one over the sum of every (row, head), from all runs of the sequence: eight lanes each
+        for (int i0 = tid / 8; i0 < (a.cq2 * H + 31) / 32 * 32; i0 += ROLE_THREADS / 8) {
+            const int i = i0 < a.cq2 * H ? i0 : a.cq2 * H - 1;
+            const float2* parts = a.part_ml + (long)s.b * a.cq2 * H + i;
+            float top = -INFINITY, sum = 0.0f;
+            for (long w = w0 + tid % 8; w <= w1; w += 32) {
+                float2 v[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) v[y] = w + 8 * y <= w1 ? parts[(w + 8 * y) * a.cq2 * H] : make_float2(-INFINITY, 0.0f);
+                const float t = fmaxf(fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)), top), ref = t == -INFINITY ? 0.0f : t;
+                sum *= fast_exp2(top - ref);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum = fmaf(v[y].y, fast_exp2(v[y].x - ref), sum);
+                top = t;
+            }
+#pragma unroll
+            for (int y = 1; y < 8; y <<= 1) {
+                const float v = __shfl_xor_sync(0xffffffffu, top, y), l = __shfl_xor_sync(0xffffffffu, sum, y);
+                const float t = fmaxf(top, v), ref = t == -INFINITY ? 0.0f : t;
+                sum = sum * fast_exp2(top - ref) + l * fast_exp2(v - ref);
+                top = t;
+            }
+            // the conv's taps of this sequence have the sums in them; a row before the first token has no keys: its probabilities are zero
+            const int row = i / H, h = i - row * H;
+            const float over = s.len - a.cq2 + row < 0 ? 0.0f : 1.0f / sum;
+            if (i0 < a.cq2 * H) {
+                if (tid % 8 == 0) top_sm[i] = s.len - a.cq2 + row < 0 ? 0.0f : top;
+                for (int j = tid % 8; j < ckp; j += 8) r_sm[(h * a.cq2 + row) * ckp + j] = t_sm[(h * a.cq2 + row) * ckp + j] * over;
+            }
+        }
+        barrier_sync(BAR_MATH, ROLE_THREADS);
+        const int limit = s.k1 < s.len ? s.k1 : s.len;
+        for (int k0 = s.k0; k0 < s.k1; k0 += tile, ++stage) {
+            // exponentials (the taps hold one over their sums), then those of the neighbours' keys that the conv reaches
+            const float* logits = a.logits + (long)s.b * a.cq2 * H * a.pitch + k0;
+#pragma unroll 4
+            for (int i = tid; i < a.cq2 * H << (a.shift - 2); i += ROLE_THREADS) {
+                const int row = i >> (a.shift - 2), kq = (i & (quads - 1)) * 4;
+                const float top = top_sm[row];
+                float4 z = make_float4(0, 0, 0, 0);
+                if (k0 + kq < s.len) z = *reinterpret_cast<const float4*>(logits + row * a.pitch + kq);
+                const float e[4] = {z.x, z.y, z.z, z.w};
+                float* p = p_sm + row * pp + left + kq;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) p[k] = k0 + kq + k < s.len ? fast_exp2(e[k] - top) : 0.0f;
+            }
+            const int beside = pp - tile;
+#pragma unroll 2
+            for (int i = tid; i < a.cq2 * H * beside; i += ROLE_THREADS) {
+                const int row = i / beside, x_ = i - row * beside, col = x_ < left ? x_ : x_ + tile, key = k0 - left + col;
+                p_sm[row * pp + col] = key >= 0 && key < s.len && col < tile + a.ck2 - 1 ? fast_exp2(logits[row * a.pitch + key - k0] - top_sm[row]) : 0.0f;
+            }
+            barrier_sync(BAR_MATH, ROLE_THREADS);
+            for (int i = tid; i < H << (a.shift - 2); i += ROLE_THREADS) {
+                const int quad = i & (quads - 1), h = i >> (a.shift - 2);
+                float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int tap = 0; tap < a.cq2; ++tap) conv_row(z, p_sm + (tap * H + h) * pp + 4 * quad, r_sm + (h * a.cq2 + tap) * ckp, ckp);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k0 + 4 * quad + e >= limit) z[e] = 0.0f;
+                *reinterpret_cast<float4*>(y_sm + (h << a.shift) + 4 * quad) = make_float4(z[0], z[1], z[2], z[3]);
+            }
+            barrier_sync(BAR_MATH, ROLE_THREADS);
+            if (stage >= 2) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
+            T* to = a_sm + (stage & 1) * a_other;
+            for (int i = tid; i < oquads << (a.shift - 2); i += ROLE_THREADS) {
+                const int kq = (i & (quads - 1)) * 4, o0 = (i >> (a.shift - 2)) * 4;
+                float z[4][4];
+                mix_heads(z, W_sm + o0, y_sm + kq, H, tile);
+#pragma unroll
+                for (int o = 0; o < 4; ++o) {
+                    if (o0 + o >= H) break;
+                    if constexpr (HALF) {
+                        float f[4][P::PIECES];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) split_pieces<T>(std::is_same_v<T, __half> ? z[o][k] * by[o0 + o] : z[o][k], f[k]);
+#pragma unroll
+                        for (int piece = 0; piece < P::PIECES; ++piece)
+                            *reinterpret_cast<uint2*>(to + ((o0 + o) * P::PIECES + piece) * ap + kq) =
+                                make_uint2(pack2<T>(f[0][piece], f[1][piece]), pack2<T>(f[2][piece], f[3][piece]));
+                    } else {
+                        *reinterpret_cast<float4*>(to + ((o0 + o) << a.shift) + kq) = make_float4(z[o][0], z[o][1], z[o][2], z[o][3]);
+                    }
+                }
+            }
+            barrier_arrive(BAR_FULL + (stage & 1), THREADS);
+        }
+        x = (long)before[s.b] + s.k1 / KEYS;
     }
 }
 
@@ -570,7 +837,7 @@ template <typename T> __global__ void __launch_bounds__(128) mta_decode_join_ker
     int *before = reinterpret_cast<int*>(smem), *lens = before + a.B + 1;
     __shared__ float sum_o[4][256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.x, b = blockIdx.y;
-    count_tiles(c, a.B, a.shift, before, lens);
+    count_tiles(c, a.B, 4, before, lens);
     __syncthreads();
     pdl_wait();
     T* out = static_cast<T*>(a.out) + ((long)b * c.H + h) * c.D;
@@ -613,13 +880,16 @@ struct Plan {
 int make_plan(Plan* p, int B, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2, int max_length) {
     const int group = H / kv_heads;
     p->gt = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
-    p->copies = 1;
-    while (H / p->gt * p->copies * 2 <= WARPS) p->copies *= 2;
     bool fits = false;
     for (p->shift = 6; p->shift >= 4 && !fits; --p->shift) {
         const int tile = 1 << p->shift;
+        // shares of a tile's units: the fewest that leave the warps least idle
+        p->copies = 1;
+        auto rounds = [&](int copies) { return (float)((H / p->gt * copies + ROLE_WARPS - 1) / ROLE_WARPS) / copies; };
+        for (int copies = 2; copies <= tile / KEYS; copies *= 2)
+            if (rounds(copies) < rounds(p->copies)) p->copies = copies;
         for (p->kv_together = kv_heads; p->kv_together >= 1 && !fits; p->kv_together = p->kv_together / 2) {
-            p->score_bytes = score_smem(B, H, group, p->kv_together, tile, cq, ck, cq2).bytes;
+            p->score_bytes = score_smem(B, H, group, kv_heads, p->kv_together, tile, cq, ck, cq2).bytes;
             p->value_bytes = value_smem(B, H, D, tile, cq2, ck2, p->copies).bytes;
             // a smaller tile before the heads are taken in parts (of whole pairs)
             fits = p->score_bytes <= SMEM_MOST && p->value_bytes <= SMEM_MOST && (p->kv_together == kv_heads || (p->shift == 4 && p->kv_together * group % 2 == 0));
@@ -628,9 +898,9 @@ int make_plan(Plan* p, int B, int H, int kv_heads, int D, int cq, int ck, int cq
         if (fits) break;
     }
     MTA_REQUIRE(fits, "mta_decode: %d heads of %d elements with kernels %dx%d and %dx%d need %zu and %zu bytes of shared memory, more than %zu", H, D, cq, ck,
-                cq2, ck2, score_smem(B, H, group, 1, 16, cq, ck, cq2).bytes, value_smem(B, H, D, 16, cq2, ck2, p->copies).bytes, SMEM_MOST);
-    const long tiles = (long)B * ((max_length + (1 << p->shift) - 1) >> p->shift);
-    const long most = (long)DECODE_SMS * 2;
+                cq2, ck2, score_smem(B, H, group, kv_heads, 1, 16, cq, ck, cq2).bytes, value_smem(B, H, D, 16, cq2, ck2, p->copies).bytes, SMEM_MOST);
+    const long tiles = (long)B * ((max_length + KEYS - 1) / KEYS);
+    const long most = DECODE_SMS;
     p->workers = (int)(tiles < most ? (tiles < 1 ? 1 : tiles) : most);
     p->pitch = (max_length + 63) / 64 * 64;
     const size_t parts = (size_t)p->workers + B;
