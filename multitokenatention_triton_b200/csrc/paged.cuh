@@ -55,10 +55,18 @@ template <> __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uin
 
 // 16 keys of one head in a warp's registers, DMAX >= D elements each.  Lane (g, t) = (lane / 4, lane % 4) holds of rows g and g + 8
 // the 16 bytes at chunk c * 64 + t * 16: whole 16-byte loads, four lanes on 64 contiguous bytes.  An mma sums over its k index in
-// any order, so the elements of a lane's 16 bytes may stand for any k as long as the queries are read the same way.
+// any order, so the elements of a lane's 16 bytes may stand for any k as long as the queries are read the same way.  The keys are the
+// B operand, two neighbouring registers of a load each; as the A operand, whose four registers would come from two loads, every
+// mma cost seven moves, and the scores of 16 keys three times as many instructions.
 template <typename T, int DMAX> struct KeyTile {
     static constexpr int CH = DMAX * (int)sizeof(T) / 64;
     static constexpr int EPL = 16 / (int)sizeof(T);      // elements in 16 bytes
+    static constexpr bool HALF = sizeof(T) == 2;
+    // Scores of ROWS query rows (a multiple of 8) in a lane's registers: value i of part p belongs to query row row_of(p, i) and key
+    // key_of(p, i) of the tile.
+    template <int ROWS> static constexpr int PARTS = HALF ? (ROWS + 15) / 16 * 2 : ROWS / 8;
+    static __device__ __forceinline__ int row_of(int p, int i, int lane) { return HALF ? p / 2 * 16 + (lane >> 2) + (i >> 1) * 8 : p * 8 + 2 * (lane & 3) + (i & 1); }
+    static __device__ __forceinline__ int key_of(int p, int i, int lane) { return HALF ? p % 2 * 8 + 2 * (lane & 3) + (i & 1) : (lane >> 2) + 8 * (i >> 1); }
     uint4 r[2][CH];
 
     // Rows base, base + 1, ... of which `live` exist; the others are zero and not read.  base < 0: none exists.  The usual whole tile
@@ -86,18 +94,21 @@ template <typename T, int DMAX> struct KeyTile {
         }
     }
 
-    // Scores of the 16 keys with NT * 8 query rows: acc[n][0..1] = key g, rows 8n + 2t, 8n + 2t + 1; acc[n][2..3] = key g + 8.
-    // 16 bits: q(n, c) gives 16 bytes (chunk c, position t) of this lane's own query row 8n + g; float32: q(row, c) of any row.
-    template <int NT, typename Q> __device__ __forceinline__ void score(float (&acc)[NT][4], int lane, Q q) const {
-        if constexpr (sizeof(T) == 2) {
+    // 16 bits: q(m, x) gives the A registers of query rows 16m + g and 16m + g + 8 for the two halves x = 2c, 2c + 1 of chunk c:
+    // {row g, row g + 8} of the half's first four bytes, then of its second.  float32: q(row, c) gives 16 bytes (chunk c, position t) of a row.
+    template <int ROWS, typename Q> __device__ __forceinline__ void score(float (&acc)[PARTS<ROWS>][4], int lane, Q q) const {
+        if constexpr (HALF) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+            for (int m = 0; m < PARTS<ROWS> / 2; ++m) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[2 * m][i] = acc[2 * m + 1][i] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    const uint4 b = q(n, c);
-                    mma_16816<T>(acc[n], r[0][c].x, r[1][c].x, r[0][c].y, r[1][c].y, b.x, b.y);
-                    mma_16816<T>(acc[n], r[0][c].z, r[1][c].z, r[0][c].w, r[1][c].w, b.z, b.w);
+                    const uint4 a0 = q(m, 2 * c), a1 = q(m, 2 * c + 1);
+                    mma_16816<T>(acc[2 * m], a0.x, a0.y, a0.z, a0.w, r[0][c].x, r[0][c].y);
+                    mma_16816<T>(acc[2 * m + 1], a0.x, a0.y, a0.z, a0.w, r[1][c].x, r[1][c].y);
+                    mma_16816<T>(acc[2 * m], a1.x, a1.y, a1.z, a1.w, r[0][c].z, r[0][c].w);
+                    mma_16816<T>(acc[2 * m + 1], a1.x, a1.y, a1.z, a1.w, r[1][c].z, r[1][c].w);
                 }
             }
         } else {
@@ -105,7 +116,7 @@ template <typename T, int DMAX> struct KeyTile {
             // and share out the rows, so that every lane has the two that the mma layout gives it
             const int t = lane & 3;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < PARTS<ROWS>; ++n) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     float2 p[2][4];                          // sums of even and odd elements

@@ -44,9 +44,13 @@ __device__ __forceinline__ long workers_of(const ConvAttnArgs& a, long n) {
 // more at 256 bytes spilled 76 bytes a thread.
 __host__ __device__ constexpr int blocks_per_sm(int row_bytes) { return row_bytes > 256 ? 2 : row_bytes > 128 ? 3 : 4; }
 
+// Queries in shared memory.  16 bits: as the A operands of the scores' mma, [16 rows][half of a chunk][lane] 16 bytes, a conflict-free load
+// each.  float32: rows, 64 bytes more than a multiple of 128 apart.
+template <typename T, int DMAX, int NT> constexpr int query_bytes = sizeof(T) == 2 ? (NT + 1) / 2 * (DMAX * 2 / 32) * 512 : NT * 8 * (DMAX * 4 + 64);
+
 // GT query heads that share a kv head, each with cq rows rounded up to pairs; NT * 8 >= all their rows of scores.
 template <typename T, int DMAX, int GT, int NT> __host__ __device__ constexpr size_t conv_attn_warp_smem(int cq, int ck) {
-    return (size_t)NT * 8 * (DMAX * sizeof(T) + 64) + (size_t)NT * 4 * RING_PITCH * 4 + (size_t)GT * ((cq + 1) / 2) * ((ck + 1) / 2 * 2) * 8 +
+    return (size_t)query_bytes<T, DMAX, NT> + (size_t)NT * 4 * RING_PITCH * 4 + (size_t)GT * ((cq + 1) / 2) * ((ck + 1) / 2 * 2) * 8 +
            (sizeof(T) == 2 ? 8 * P_PITCH * 2 : GT * KEYS * 4);
 }
 
@@ -61,10 +65,9 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int cqp = (a.cq + 1) / 2, ckp = (a.ck + 1) / 2 * 2;
     char* mine = smem + warp * conv_attn_warp_smem<T, DMAX, GT, NT>(a.cq, a.ck);
-    // row pitch of the queries: 64 bytes more than a multiple of 128, so that rows g and g + 1 of an 8-lane phase miss each other's banks
-    constexpr int QP = DMAX * (int)sizeof(T) + 64;
+    constexpr int QP = DMAX * (int)sizeof(T) + 64, QROWS = HALF ? (NT + 1) / 2 * 16 : NT * 8;
     char* q_sm = mine;
-    float* s_sm = reinterpret_cast<float*>(mine + NT * 8 * QP);
+    float* s_sm = reinterpret_cast<float*>(mine + query_bytes<T, DMAX, NT>);
     float2* w_sm = reinterpret_cast<float2*>(s_sm + NT * 4 * RING_PITCH);       // [head][pair of tap rows][key tap]
     T* p_sm = reinterpret_cast<T*>(w_sm + GT * cqp * ckp);                      // [column][key]; float32: [head][key]
     int* before = reinterpret_cast<int*>(smem + WARPS * conv_attn_warp_smem<T, DMAX, GT, NT>(a.cq, a.ck));
@@ -106,12 +109,18 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
         values.load(v_pool, key_base(u0), live(u0), c.D, lane);
 
         // queries and taps of this line
-        for (int i = lane; i < NT * 8 * (DMAX / EPL); i += 32) {
+        for (int i = lane; i < QROWS * (DMAX / EPL); i += 32) {
             const int row = i / (DMAX / EPL), e = (i % (DMAX / EPL)) * EPL, gq = row / (2 * cqp), tap = row % (2 * cqp), pos = len - a.cq + tap;
             uint4 u = make_uint4(0, 0, 0, 0);
             if (gq < GT && tap < a.cq && pos >= 0 && e < c.D)
                 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(c.q_hist) + (((long)slot * c.ring + pos % c.ring) * c.H + h0 + gq) * c.D + e);
-            *reinterpret_cast<uint4*>(q_sm + row * QP + e * (int)sizeof(T)) = u;
+            if constexpr (HALF) {
+                // 16 bytes of a row: the first two registers of one half of the chunk, then of the other, for lane (row % 8, position)
+                uint32_t* to = reinterpret_cast<uint32_t*>(q_sm + ((row / 16 * K::CH + e / 32) * 2 * 32 + row % 8 * 4 + e / 8 % 4) * 16) + row / 8 % 2;
+                to[0] = u.x; to[2] = u.y; to[128] = u.z; to[130] = u.w;
+            } else {
+                *reinterpret_cast<uint4*>(q_sm + row * QP + e * (int)sizeof(T)) = u;
+            }
         }
         for (int i = lane; i < GT * cqp * ckp; i += 32) {
             const int j = i % ckp, pair = i / ckp % cqp, y = i / ckp / cqp;
@@ -134,27 +143,31 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
             for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
 
         for (int u = u0 - 1; u <= u1; ++u) {
-            float acc[NT][4];
-            keys.template score<NT>(acc, lane, [&](int row, int ch) {
-                return *reinterpret_cast<const uint4*>(q_sm + (HALF ? 8 * row + g : row) * QP + ch * 64 + t4 * 16);
+            constexpr int PARTS = K::template PARTS<NT * 8>;
+            float acc[PARTS][4];
+            keys.template score<NT * 8>(acc, lane, [&](int row, int ch) {
+                if constexpr (HALF) return reinterpret_cast<const uint4*>(q_sm)[(row * 2 * K::CH + ch) * 32 + lane];
+                else return *reinterpret_cast<const uint4*>(q_sm + row * QP + ch * 64 + t4 * 16);
             });
             if (u < u1) keys.load(k_pool, key_base(u + 1), live(u + 1), c.D, lane);
             const int col = ((u + 3) % 3) * KEYS + shift;
             // scores above the diagonal are zero; those of tiles outside the sequence are zero already
             if (u * KEYS + KEYS - 1 > len - a.cq) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        if (u * KEYS + g + 8 * (y >> 1) > len - a.cq + (8 * nt + 2 * t4 + (y & 1)) % (2 * cqp)) acc[nt][y] = 0.0f;
+                    for (int i = 0; i < 4; ++i)
+                        if (u * KEYS + K::key_of(p, i, lane) > len - a.cq + K::row_of(p, i, lane) % (2 * cqp)) acc[p][i] = 0.0f;
             }
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                int at = col + g + 8 * y;
-                if (at >= RING) at -= RING;
+            for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    *reinterpret_cast<float2*>(s_sm + (4 * nt + t4) * RING_PITCH + 2 * at) = make_float2(acc[nt][2 * y], acc[nt][2 * y + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    const int row = K::row_of(p, i, lane);
+                    int at = col + K::key_of(p, i, lane);
+                    if (at >= RING) at -= RING;
+                    if (row < NT * 8) s_sm[(row >> 1) * RING_PITCH + 2 * at + (row & 1)] = acc[p][i];
+                }
             }
             __syncwarp();
             if (u > u0) {

@@ -177,6 +177,33 @@ struct Pages {
     }
 };
 
+// Whether two tiles of keys or values are in flight in a warp's registers.  One at a time left the memory at 3.4 TB/s.
+template <typename T, int DMAX> constexpr bool TWO_IN_FLIGHT = sizeof(T) * DMAX <= 256;
+
+// fetch(tile, task) starts the loads of the next task, work(tile, task) does a task and fetches another into the same registers; both say
+// whether there is one.
+template <typename TILE, typename TASK, bool TWO, typename FETCH, typename WORK> __device__ __forceinline__ void in_turns(FETCH& fetch, WORK& work) {
+    TILE a;
+    TASK ta;
+    bool on_a = fetch(a, ta);
+    if constexpr (TWO) {
+        TILE b;
+        TASK tb;
+        bool on_b = fetch(b, tb);
+        while (on_a) {
+            on_a = work(a, ta);
+            if (!on_b) break;
+            on_b = work(b, tb);
+        }
+    } else {
+        while (on_a) on_a = work(a, ta);
+    }
+}
+
+// The registers of a block are dealt anew once the roles part: 168 to a thread of the memory half, 88 to one of the other, 128 * 512 in all.
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+
 template <typename T, int DMAX, int NT>
 __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCache c, MtaArgs a) {
     constexpr bool HALF = sizeof(T) == 2;
@@ -205,45 +232,34 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
 
     if (warp < ROLE_WARPS) {
         // ---- scores.  A stage is a tile and a group of heads; a task one kv head and 16 keys of it.
+        more_registers();
         const T* pool = static_cast<const T*>(c.k);
         const T* queries = static_cast<const T*>(c.q_hist);
+        const int head_stride = c.D << c.page_shift;
         long* q_at = reinterpret_cast<long*>(smem + m.q_at) + warp * DECODE_MAX_ROWS;       // this warp's query rows
-        // Where the loads are: one task ahead of the arithmetic.  Of the tasks behind that, L2 is asked a stage ahead.
+        // Where the loads are: two tasks ahead of the arithmetic, one where a row is too wide for that.
         struct Cursor {
             Span s;
             long at;           // of this lane's unit
-            int k0, hk0, first, units, hk, unit, tasks_left, taken, stage, turn;
+            int k0, hk0, first, units, hk, unit, tasks_left, stage, turn, place;
             Pages next;
             bool done;
         } cur = {};
         auto first_of = [&](int k0) { return k0 + (whole && k0 > cur.s.k0 ? hr : -hl); };
         auto units_of = [&](int k0) { return ((k0 + tile < cur.s.k1 ? k0 + tile : cur.s.k1) + hr - first_of(k0)) / KEYS; };
-        // L2 is asked for this warp's tasks of the tile at k0, a task per lane; `at` is the place of the lane's unit.
-        auto ask_l2 = [&](int k0, long at) {
-            const int units = units_of(k0), nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together;
-            const int t0 = warp * nk * units / ROLE_WARPS, t1 = (warp + 1) * nk * units / ROLE_WARPS;
-            for (int t = t0; t < t1; t += 32) {
-                const int mine = t + lane < t1 ? t + lane : t1 - 1, hk = mine / units, unit = mine - hk * units;
-                const long base = __shfl_sync(0xffffffffu, at, unit);
-                const int live = cur.s.len - (first_of(k0) + unit * KEYS);
-                if (t + lane < t1 && base >= 0)
-                    prefetch_l2(pool + base + ((long)(cur.hk0 + hk) << c.page_shift) * c.D, (uint32_t)((live < KEYS ? live : KEYS) * c.D * sizeof(T)));
-            }
-        };
         auto enter_stage = [&] {
             cur.first = first_of(cur.k0);
             cur.units = units_of(cur.k0);
+            cur.place = (cur.first + cur.turn) % ring.keys;
             const int nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together, tasks = nk * cur.units;
             const int t0 = warp * tasks / ROLE_WARPS;
             cur.tasks_left = (warp + 1) * tasks / ROLE_WARPS - t0;
-            cur.taken = 0;
             cur.hk = t0 / cur.units;
             cur.unit = t0 - cur.hk * cur.units;
             const int key = cur.first + lane * KEYS;
             const bool on = lane < cur.units && key >= 0 && key < cur.s.len;
             if (!whole || cur.k0 == cur.s.k0) cur.next.look_up(c, cur.s.slot, key, on);
             cur.at = cur.next.at(c, key, on);
-            if (!whole || cur.k0 == cur.s.k0) ask_l2(cur.k0, cur.at);
             if (whole) {                                         // the next tile of the span
                 const int ahead = cur.k0 + tile + hr + lane * KEYS;
                 cur.next.look_up(c, cur.s.slot, ahead, lane < tile / KEYS && ahead < cur.s.len);
@@ -257,9 +273,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
         };
         enter_span(begin, 0);
         enter_stage();
-        K keys;
-        int key = 0, hk = 0;                                     // of the task whose keys are on their way
-        auto fetch = [&]() -> bool {
+        struct Task {
+            int key, place, hk, hk0, stage, b, len, slot;
+        };
+        // The next task of this warp, its keys on their way into `keys`.
+        auto fetch = [&](K& keys, Task& t) -> bool {
             while (!cur.done && cur.tasks_left == 0) {
                 ++cur.stage;
                 cur.hk0 += a.kv_together;
@@ -276,86 +294,91 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             }
             if (cur.done) return false;
             const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
-            key = cur.first + cur.unit * KEYS;
-            hk = cur.hk0 + cur.hk;
-            keys.load(pool, base < 0 ? base : base + ((long)hk << c.page_shift) * c.D, cur.s.len - key, c.D, lane);
+            t.key = cur.first + cur.unit * KEYS;
+            t.hk0 = cur.hk0; t.hk = cur.hk0 + cur.hk; t.stage = cur.stage;
+            t.place = cur.place + cur.unit * KEYS;
+            if (t.place >= ring.keys) t.place -= ring.keys;
+            t.b = cur.s.b; t.len = cur.s.len; t.slot = cur.s.slot;
+            keys.load(pool, base < 0 ? base : base + (long)t.hk * head_stride, t.len - t.key, c.D, lane);
             if (++cur.unit == cur.units) { cur.unit = 0; ++cur.hk; }
             --cur.tasks_left;
-            if (++cur.taken == 2 && whole && cur.k0 + tile < cur.s.k1) {
-                const int ahead = cur.k0 + tile + hr + lane * KEYS;
-                ask_l2(cur.k0 + tile, cur.next.at(c, ahead, lane < tile / KEYS && ahead < cur.s.len));
-            }
             return true;
         };
         int stage = 0, span_b = -1, q_head = -1;
-        uint4 q[HALF ? NT : 1][HALF ? K::CH : 1];
-        for (bool more = fetch(); more;) {
-            // the cursor still stands where this task's keys were fetched
-            while (stage < cur.stage) {
+        constexpr int PARTS = K::template PARTS<NT * 8>;
+        uint4 q[HALF ? PARTS / 2 : 1][HALF ? 2 * K::CH : 1];     // the A operands of a head
+        // Scores of one task into the ring; the registers of its keys take the keys of a later one as soon as they are free.
+        auto work = [&](K& keys, Task& t) -> bool {
+            while (stage < t.stage) {
                 barrier_arrive(BAR_FULL + (stage & 1), THREADS);
                 ++stage;
                 if (stage >= 2) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
             }
-            const int len = cur.s.len;
-            if (cur.s.b != span_b) {
+            const int len = t.len;
+            if (t.b != span_b) {
                 __syncwarp();
                 const int pos = len - R + lane;
-                q_at[lane] = lane < R && pos >= 0 ? ((long)cur.s.slot * c.ring + pos % c.ring) * H * c.D : -1;
-                span_b = cur.s.b;
+                q_at[lane] = lane < R && pos >= 0 ? ((long)t.slot * c.ring + pos % c.ring) * H * c.D : -1;
+                span_b = t.b;
                 q_head = -1;
                 __syncwarp();
             }
-            const bool full = key + KEYS - 1 <= len - R;                             // every row sees every key
-            const int now = key, local = (hk - cur.hk0) * group, head0 = hk * group;
-            const int at = (now + cur.turn + shift) % ring.keys + g;                 // ring position of key `g` of the unit
-            float* buf = s_sm + (stage & 1) * s_other + 2 * t4 * ring.row;
+            bool more = true;
+            const bool full = t.key + KEYS - 1 <= len - R;                           // every row sees every key
+            const int now = t.key, local = (t.hk - t.hk0) * group, head0 = t.hk * group;
+            const int at = t.place + shift;                                          // ring position of the first key
+            float* buf = s_sm + (stage & 1) * s_other;
             for (int gq = 0; gq < group; ++gq) {
                 const T* qh = queries + (long)(head0 + gq) * c.D;
-                float acc[NT][4];
+                float acc[PARTS][4];
                 if constexpr (HALF) {
                     if (q_head != head0 + gq) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const long row = q_at[8 * nt + g];
+                        for (int m_ = 0; m_ < PARTS / 2; ++m_) {
+                            const long r0 = q_at[16 * m_ + g], r1 = NT > 1 ? q_at[16 * m_ + 8 + g] : -1;
 #pragma unroll
                             for (int ch = 0; ch < K::CH; ++ch) {
                                 const int e = (ch * 4 + t4) * K::EPL;
-                                q[nt][ch] = make_uint4(0, 0, 0, 0);
-                                if (row >= 0 && e < c.D) q[nt][ch] = __ldg(reinterpret_cast<const uint4*>(qh + row + e));
+                                uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+                                if (r0 >= 0 && e < c.D) lo = __ldg(reinterpret_cast<const uint4*>(qh + r0 + e));
+                                if (r1 >= 0 && e < c.D) hi = __ldg(reinterpret_cast<const uint4*>(qh + r1 + e));
+                                q[m_][2 * ch] = make_uint4(lo.x, hi.x, lo.y, hi.y);
+                                q[m_][2 * ch + 1] = make_uint4(lo.z, hi.z, lo.w, hi.w);
                             }
                         }
                         q_head = head0 + gq;
                     }
-                    keys.template score<NT>(acc, lane, [&](int nt, int ch) { return q[nt][ch]; });
+                    keys.template score<NT * 8>(acc, lane, [&](int m_, int x) { return q[m_][x]; });
                 } else {
-                    keys.template score<NT>(acc, lane, [&](int row, int ch) {
+                    keys.template score<NT * 8>(acc, lane, [&](int row, int ch) {
                         const long r = q_at[row];
                         const int e = (ch * 4 + t4) * K::EPL;
                         return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
                     });
                 }
-                if (gq == group - 1) more = fetch();
+                if (gq == group - 1) more = fetch(keys, t);
                 float* s = buf + ((local + gq) >> 1) * R * ring.row + ((local + gq) & 1);
                 if (!full) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                        for (int y = 0; y < 4; ++y)
-                            if (now + g + 8 * (y >> 1) > len - R + 8 * nt + 2 * t4 + (y & 1)) acc[nt][y] = 0.0f;
+                        for (int i = 0; i < 4; ++i)
+                            if (now + K::key_of(p, i, lane) > len - R + K::row_of(p, i, lane)) acc[p][i] = 0.0f;
                 }
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    int pos = at + 8 * y;
-                    if (pos >= ring.keys) pos -= ring.keys;
-                    float* to = s + (pos & ~3) + (pos & 1) * 2 + (pos & 2 ? ring.half : 0);
+                for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (8 * nt + 2 * t4 < R) to[8 * nt * ring.row] = acc[nt][2 * y];
-                        if (8 * nt + 2 * t4 + 1 < R) to[(8 * nt + 1) * ring.row] = acc[nt][2 * y + 1];
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = K::row_of(p, i, lane);
+                        int pos = at + K::key_of(p, i, lane);
+                        if (pos >= ring.keys) pos -= ring.keys;
+                        if (row < R) s[row * ring.row + (pos & ~3) + (pos & 1) * 2 + (pos & 2 ? ring.half : 0)] = acc[p][i];
                     }
                 }
             }
-        }
+            return more;
+        };
+        in_turns<K, Task, TWO_IN_FLIGHT<T, DMAX>>(fetch, work);
         // stages behind this warp's last task: the cursor stands behind the run's last stage
         while (stage < cur.stage) {
             barrier_arrive(BAR_FULL + (stage & 1), THREADS);
@@ -366,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     }
 
     // ---- conv, head mix, softmax statistics
+    fewer_registers();
     const int tid = threadIdx.x - ROLE_THREADS;
     load_mix(W_sm, a.W1, H, a.w_dtype);
     for (int i = tid; i < (H + 1) / 2 * a.cq * ckp; i += ROLE_THREADS) {
@@ -498,12 +522,14 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
 
     if (warp >= ROLE_WARPS) {
         // ---- product with the values.  A stage is a tile; the loads run ahead of the arithmetic as in the scores kernel.
+        more_registers();
         const int tid = threadIdx.x - ROLE_THREADS, me_warp = warp - ROLE_WARPS, tasks = H / GT * copies;
         const T* pool = static_cast<const T*>(c.v);
+        const int head_stride = c.D << c.page_shift;
         struct Cursor {
             Span s;
             long at;
-            int k0, units, task, unit, last, taken, stage;
+            int k0, units, task, unit, last, stage;
             Pages next;
             bool done;
         } cur = {};
@@ -512,26 +538,14 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
             cur.unit = copy * all / copies;
             cur.last = (copy + 1) * all / copies < cur.units ? (copy + 1) * all / copies : cur.units;
         };
-        // L2 is asked for the tile at k0, a (kv head, unit) per thread of this half; `at` is the place of the lane's unit.
-        auto ask_l2 = [&](int k0, long at) {
-            const int units = ((k0 + tile < cur.s.k1 ? k0 + tile : cur.s.k1) - k0) / KEYS, all = c.kv_heads * units;
-            for (int t = me_warp * 32; t < all; t += ROLE_THREADS) {
-                const int mine = t + lane < all ? t + lane : all - 1, hk = mine / units, unit = mine - hk * units;
-                const long base = __shfl_sync(0xffffffffu, at, unit);
-                const int live = cur.s.len - (k0 + unit * KEYS);
-                if (t + lane < all && base >= 0) prefetch_l2(pool + base + ((long)hk << c.page_shift) * c.D, (uint32_t)((live < KEYS ? live : KEYS) * c.D * sizeof(T)));
-            }
-        };
         auto enter_stage = [&] {
             cur.units = ((cur.k0 + tile < cur.s.k1 ? cur.k0 + tile : cur.s.k1) - cur.k0) / KEYS;
             const int key = cur.k0 + lane * KEYS;
             const bool on = lane < cur.units && key < cur.s.len;
             if (cur.k0 == cur.s.k0) cur.next.look_up(c, cur.s.slot, key, on);
             cur.at = cur.next.at(c, key, on);
-            if (cur.k0 == cur.s.k0) ask_l2(cur.k0, cur.at);
             const bool ahead = lane < tile / KEYS && key + tile < cur.s.len;
             cur.next.look_up(c, cur.s.slot, key + tile, ahead);
-            cur.taken = 0;
             cur.task = me_warp;
             share();
         };
@@ -541,10 +555,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         };
         enter_span(begin);
         enter_stage();
-        V values;
-        int t_task = 0, t_unit = 0;                              // whose values are on their way
-        bool t_first = false, t_final = false;                   // of its task and stage
-        auto fetch = [&]() -> bool {
+        struct Task {
+            int task, unit, stage;
+            bool first, final;     // of its task and stage
+        };
+        auto fetch = [&](V& values, Task& t) -> bool {
             while (!cur.done && (cur.task >= tasks || cur.unit >= cur.last)) {
                 if (cur.task < tasks) {
                     cur.task += ROLE_WARPS;
@@ -563,14 +578,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
             if (cur.done) return false;
             const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
             const int copy = cur.task % copies, hk = cur.task / copies * GT / group;
-            t_task = cur.task; t_unit = cur.unit;
-            t_first = cur.unit == copy * (tile / KEYS) / copies;
-            values.load(pool, base < 0 ? base : base + ((long)hk << c.page_shift) * c.D, cur.s.len - (cur.k0 + cur.unit * KEYS), c.D, lane);
-            t_final = ++cur.unit == cur.last;
-            if (++cur.taken == 2 && cur.k0 + tile < cur.s.k1) {
-                const int ahead = cur.k0 + tile + lane * KEYS;
-                ask_l2(cur.k0 + tile, cur.next.at(c, ahead, lane < tile / KEYS && ahead < cur.s.len));
-            }
+            t.task = cur.task; t.unit = cur.unit; t.stage = cur.stage;
+            t.first = cur.unit == copy * (tile / KEYS) / copies;
+            values.load(pool, base < 0 ? base : base + (long)hk * head_stride, cur.s.len - (cur.k0 + cur.unit * KEYS), c.D, lane);
+            t.final = ++cur.unit == cur.last;
             return true;
         };
         int stage = 0, stages = 0;
@@ -619,13 +630,13 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         };
         barrier_sync(BAR_MEMORY, ROLE_THREADS);                  // the outputs are zero
         bool started = false;
-        for (bool more = fetch(); more;) {
-            // the cursor still stands where this task's values were fetched
+        auto work = [&](V& values, Task& t) -> bool {
             if (!started) barrier_sync(BAR_FULL, THREADS);       // the first stage
             started = true;
-            pass_stages(cur.stage);
-            const int unit = t_unit, copy = t_task % copies, h0 = t_task / copies * GT;
-            const bool first = t_first, final = t_final;
+            pass_stages(t.stage);
+            const int unit = t.unit, copy = t.task % copies, h0 = t.task / copies * GT;
+            const bool first = t.first, final = t.final;
+            bool more = true;
             const T* weights = a_sm + (stage & 1) * a_other;
             if (first) {
 #pragma unroll
@@ -638,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 const bool on = y < GT && piece < P::PIECES;
                 const uint32_t* col = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4 + unit * 8;
                 values.multiply(acc, on ? col[0] : 0u, on ? col[4] : 0u);
-                more = fetch();
+                more = fetch(values, t);
                 if (final) {
                     // sum over the pieces; a head's columns are those of one lane (four heads) or of two, which then halve the elements
                     const int head = h0 + t4 * 2 / P::STRIDE;
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                         for (int e = 0; e < 4; ++e) acc[y][0][e] = fmaf(p, f[e], acc[y][0][e]);
                     }
                 }
-                more = fetch();
+                more = fetch(values, t);
                 if (final) {
                     const int e0 = (lane % V::ROWLANES) * 4;
 #pragma unroll
@@ -705,13 +716,16 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                     }
                 }
             }
-        }
+            return more;
+        };
+        in_turns<V, Task, TWO_IN_FLIGHT<T, DMAX>>(fetch, work);
         if (!started) barrier_sync(BAR_FULL, THREADS);           // no task at all
         pass_stages(stages);
         return;
     }
 
     // ---- probabilities, conv, head mix: the weights of the values
+    fewer_registers();
     const int tid = threadIdx.x;
     load_mix(W_sm, a.W2, H, a.w_dtype);
     for (int i = tid; i < H * a.cq2 * ckp; i += ROLE_THREADS) {
