@@ -49,6 +49,9 @@ __host__ __device__ inline int halo(int x) { return (x + KEYS - 1) / KEYS * KEYS
 // where the one before ended.  Where not all heads fit, the tiles (of one group of heads after another) have a ring each.  Two heads stand side by side, which lets one packed FMA serve both.  Keys (4i, 4i + 1) lie in the first half of a
 // row, (4i + 2, 4i + 3) in the second, 16 bytes each: the conv's threads, four keys apart, read neighbouring 16 bytes.  The pads
 // put the rows and halves that an accumulator writes at once into different banks.
+// Windows begin on multiples of four keys: taps have up to three zeros in front (`lead`) for that, and zeros behind up to `taps`.
+__host__ __device__ inline int lead(int ck) { return (4 - (ck - 1) / 2 % 4) % 4; }
+__host__ __device__ inline int score_taps(int ck) { return round4(ck + lead(ck)); }
 struct ScoreRing {
     int keys, half, row;   // floats of half a row and of a row
     __host__ __device__ ScoreRing(int tile, int ck, bool whole) {
@@ -71,7 +74,7 @@ __host__ __device__ inline ScoreSmem score_smem(int B, int H, int group, int kv_
     m.s = at; at += m.s_one * (whole ? 1 : 2);
     m.c = at; at += (size_t)cq2 * H * tile * 4;
     m.W = at; at += (size_t)H * round4(H) * 4;
-    m.taps = at; at += (size_t)((H + 1) / 2) * cq * round4(ck) * 8;
+    m.taps = at; at += (size_t)((H + 1) / 2) * cq * score_taps(ck) * 8;
     m.ml = at; at += (size_t)cq2 * H * (tile / 4) * 8;
     m.q_at = at; at += (size_t)ROLE_WARPS * DECODE_MAX_ROWS * 8;
     m.before = at; at += (size_t)(2 * B + 1) * 4;
@@ -177,28 +180,9 @@ struct Pages {
     }
 };
 
-// Whether two tiles of keys or values are in flight in a warp's registers.  One at a time left the memory at 3.4 TB/s.
-template <typename T, int DMAX> constexpr bool TWO_IN_FLIGHT = sizeof(T) * DMAX <= 256;
-
-// fetch(tile, task) starts the loads of the next task, work(tile, task) does a task and fetches another into the same registers; both say
-// whether there is one.
-template <typename TILE, typename TASK, bool TWO, typename FETCH, typename WORK> __device__ __forceinline__ void in_turns(FETCH& fetch, WORK& work) {
-    TILE a;
-    TASK ta;
-    bool on_a = fetch(a, ta);
-    if constexpr (TWO) {
-        TILE b;
-        TASK tb;
-        bool on_b = fetch(b, tb);
-        while (on_a) {
-            on_a = work(a, ta);
-            if (!on_b) break;
-            on_b = work(b, tb);
-        }
-    } else {
-        while (on_a) on_a = work(a, ta);
-    }
-}
+// Tiles of 16 keys or values that a warp's task has and its registers hold in flight: as many as fit.  One at a time left the memory at
+// 3.4 TB/s, and what a task costs besides its loads and products is paid half as often.
+template <typename T, int DMAX> constexpr int TOGETHER = sizeof(T) * DMAX <= 256 ? 2 : 1;
 
 // The registers of a block are dealt anew once the roles part: 168 to a thread of the memory half, 88 to one of the other, 128 * 512 in all.
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
@@ -210,9 +194,8 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     using K = KeyTile<T, DMAX>;
     extern __shared__ __align__(16) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = round4(a.ck);
-    const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo(a.ck - 1 - left);
-    const int shift = left & 3;                                  // puts the windows of a tile's quads of keys on 16-byte boundaries
+    const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = score_taps(a.ck);
+    const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo(a.ck - 1 - left), first_tap = lead(a.ck);
     const bool whole = a.kv_together == c.kv_heads;              // all heads at once: what tiles share stays in the ring
     const ScoreRing ring(tile, a.ck, whole);
     const ScoreSmem m = score_smem(a.B, H, group, c.kv_heads, a.kv_together, tile, a.cq, a.ck, a.cq2);
@@ -231,13 +214,14 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     const long begin = run_begin(me, n, workers), end = run_begin(me + 1, n, workers);
 
     if (warp < ROLE_WARPS) {
-        // ---- scores.  A stage is a tile and a group of heads; a task one kv head and 16 keys of it.
+        // ---- scores.  A stage is a tile and a group of heads; a task one kv head and 16 or 32 keys of it.
         more_registers();
         const T* pool = static_cast<const T*>(c.k);
         const T* queries = static_cast<const T*>(c.q_hist);
         const int head_stride = c.D << c.page_shift;
+        constexpr int N = TOGETHER<T, DMAX>;
         long* q_at = reinterpret_cast<long*>(smem + m.q_at) + warp * DECODE_MAX_ROWS;       // this warp's query rows
-        // Where the loads are: two tasks ahead of the arithmetic, one where a row is too wide for that.
+        // Where the loads are, one task ahead of the arithmetic.
         struct Cursor {
             Span s;
             long at;           // of this lane's unit
@@ -251,11 +235,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             cur.first = first_of(cur.k0);
             cur.units = units_of(cur.k0);
             cur.place = (cur.first + cur.turn) % ring.keys;
-            const int nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together, tasks = nk * cur.units;
-            const int t0 = warp * tasks / ROLE_WARPS;
+            const int nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together;
+            const int per_head = (cur.units + N - 1) / N, tasks = nk * per_head, t0 = warp * tasks / ROLE_WARPS;
             cur.tasks_left = (warp + 1) * tasks / ROLE_WARPS - t0;
-            cur.hk = t0 / cur.units;
-            cur.unit = t0 - cur.hk * cur.units;
+            cur.hk = t0 / per_head;
+            cur.unit = (t0 - cur.hk * per_head) * N;
             const int key = cur.first + lane * KEYS;
             const bool on = lane < cur.units && key >= 0 && key < cur.s.len;
             if (!whole || cur.k0 == cur.s.k0) cur.next.look_up(c, cur.s.slot, key, on);
@@ -273,11 +257,9 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
         };
         enter_span(begin, 0);
         enter_stage();
-        struct Task {
-            int key, place, hk, hk0, stage, b, len, slot;
-        };
-        // The next task of this warp, its keys on their way into `keys`.
-        auto fetch = [&](K& keys, Task& t) -> bool {
+        K keys[N];
+        int task_unit = 0, task_hk = 0;                          // whose keys are on their way
+        auto fetch = [&]() -> bool {
             while (!cur.done && cur.tasks_left == 0) {
                 ++cur.stage;
                 cur.hk0 += a.kv_together;
@@ -293,44 +275,49 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                 enter_stage();
             }
             if (cur.done) return false;
-            const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
-            t.key = cur.first + cur.unit * KEYS;
-            t.hk0 = cur.hk0; t.hk = cur.hk0 + cur.hk; t.stage = cur.stage;
-            t.place = cur.place + cur.unit * KEYS;
-            if (t.place >= ring.keys) t.place -= ring.keys;
-            t.b = cur.s.b; t.len = cur.s.len; t.slot = cur.s.slot;
-            keys.load(pool, base < 0 ? base : base + (long)t.hk * head_stride, t.len - t.key, c.D, lane);
-            if (++cur.unit == cur.units) { cur.unit = 0; ++cur.hk; }
+            task_unit = cur.unit;
+            task_hk = cur.hk;
+            const long head = (long)(cur.hk0 + cur.hk) * head_stride;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int u = cur.unit + i;
+                const long base = __shfl_sync(0xffffffffu, cur.at, u);       // -1 behind the last unit
+                keys[i].load(pool, base < 0 ? base : base + head, cur.s.len - (cur.first + u * KEYS), c.D, lane);
+            }
+            cur.unit += N;
+            if (cur.unit >= cur.units) { cur.unit = 0; ++cur.hk; }
             --cur.tasks_left;
             return true;
         };
         int stage = 0, span_b = -1, q_head = -1;
         constexpr int PARTS = K::template PARTS<NT * 8>;
         uint4 q[HALF ? PARTS / 2 : 1][HALF ? 2 * K::CH : 1];     // the A operands of a head
-        // Scores of one task into the ring; the registers of its keys take the keys of a later one as soon as they are free.
-        auto work = [&](K& keys, Task& t) -> bool {
-            while (stage < t.stage) {
+        // Scores of one task into the ring; the registers of its keys take the next task's as soon as they are free.
+        for (bool more = fetch(); more;) {
+            // the cursor still stands where this task's keys were fetched
+            while (stage < cur.stage) {
                 barrier_arrive(BAR_FULL + (stage & 1), THREADS);
                 ++stage;
                 if (stage >= 2) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
             }
-            const int len = t.len;
-            if (t.b != span_b) {
+            const int len = cur.s.len;
+            if (cur.s.b != span_b) {
                 __syncwarp();
                 const int pos = len - R + lane;
-                q_at[lane] = lane < R && pos >= 0 ? ((long)t.slot * c.ring + pos % c.ring) * H * c.D : -1;
-                span_b = t.b;
+                q_at[lane] = lane < R && pos >= 0 ? ((long)cur.s.slot * c.ring + pos % c.ring) * H * c.D : -1;
+                span_b = cur.s.b;
                 q_head = -1;
                 __syncwarp();
             }
-            bool more = true;
-            const bool full = t.key + KEYS - 1 <= len - R;                           // every row sees every key
-            const int now = t.key, local = (t.hk - t.hk0) * group, head0 = t.hk * group;
-            const int at = t.place + shift;                                          // ring position of the first key
+            const int first_key = cur.first + task_unit * KEYS, local = task_hk * group, head0 = (cur.hk0 + task_hk) * group;
+            const int units = cur.units - task_unit;                                 // of this task, if less than N
+            int place = cur.place + task_unit * KEYS;
+            if (place >= ring.keys) place -= ring.keys;
+            const bool full = first_key + N * KEYS - 1 <= len - R;                   // every row sees every key
             float* buf = s_sm + (stage & 1) * s_other;
             for (int gq = 0; gq < group; ++gq) {
                 const T* qh = queries + (long)(head0 + gq) * c.D;
-                float acc[PARTS][4];
+                float acc[N][PARTS][4];
                 if constexpr (HALF) {
                     if (q_head != head0 + gq) {
 #pragma unroll
@@ -348,37 +335,43 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                         }
                         q_head = head0 + gq;
                     }
-                    keys.template score<NT * 8>(acc, lane, [&](int m_, int x) { return q[m_][x]; });
+#pragma unroll
+                    for (int i = 0; i < N; ++i) keys[i].template score<NT * 8>(acc[i], lane, [&](int m_, int x) { return q[m_][x]; });
                 } else {
-                    keys.template score<NT * 8>(acc, lane, [&](int row, int ch) {
-                        const long r = q_at[row];
-                        const int e = (ch * 4 + t4) * K::EPL;
-                        return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
-                    });
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        keys[i].template score<NT * 8>(acc[i], lane, [&](int row, int ch) {
+                            const long r = q_at[row];
+                            const int e = (ch * 4 + t4) * K::EPL;
+                            return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
+                        });
                 }
-                if (gq == group - 1) more = fetch(keys, t);
+                if (gq == group - 1) more = fetch();
                 float* s = buf + ((local + gq) >> 1) * R * ring.row + ((local + gq) & 1);
-                if (!full) {
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
+                for (int i = 0; i < N; ++i) {
+                    if (i > 0 && i >= units) break;
+                    const int key = first_key + i * KEYS;
+                    if (!full) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (now + K::key_of(p, i, lane) > len - R + K::row_of(p, i, lane)) acc[p][i] = 0.0f;
-                }
+                        for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
+                            for (int y = 0; y < 4; ++y)
+                                if (key + K::key_of(p, y, lane) > len - R + K::row_of(p, y, lane)) acc[i][p][y] = 0.0f;
+                    }
+                    float* to = s + (place + i * KEYS >= ring.keys ? place + i * KEYS - ring.keys : place + i * KEYS);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = K::row_of(p, i, lane);
-                        int pos = at + K::key_of(p, i, lane);
-                        if (pos >= ring.keys) pos -= ring.keys;
-                        if (row < R) s[row * ring.row + (pos & ~3) + (pos & 1) * 2 + (pos & 2 ? ring.half : 0)] = acc[p][i];
+                    for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            if (HALF && y >= 2 && NT == 1) continue;                 // rows 8 to 15
+                            const int row = K::row_of(p, y, lane), kk = K::key_of(p, y, lane);
+                            if (row < R) to[row * ring.row + (kk & ~3) + (kk & 1) * 2 + (kk & 2 ? ring.half : 0)] = acc[i][p][y];
+                        }
                     }
                 }
             }
-            return more;
-        };
-        in_turns<K, Task, TWO_IN_FLIGHT<T, DMAX>>(fetch, work);
+        }
         // stages behind this warp's last task: the cursor stands behind the run's last stage
         while (stage < cur.stage) {
             barrier_arrive(BAR_FULL + (stage & 1), THREADS);
@@ -393,10 +386,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     const int tid = threadIdx.x - ROLE_THREADS;
     load_mix(W_sm, a.W1, H, a.w_dtype);
     for (int i = tid; i < (H + 1) / 2 * a.cq * ckp; i += ROLE_THREADS) {
-        const int j = i % ckp, row = i / ckp, tap = row % a.cq, h = row / a.cq * 2;
+        const int j = i % ckp - first_tap, row = i / ckp, tap = row % a.cq, h = row / a.cq * 2;
         const long at = ((long)h * a.cq + tap) * a.ck + j;
-        t_sm[i] = make_float2(j < a.ck ? load_weight(a.w1, at, a.w_dtype) * a.scale : 0.0f,
-                              j < a.ck && h + 1 < H ? load_weight(a.w1, at + a.cq * a.ck, a.w_dtype) * a.scale : 0.0f);
+        t_sm[i] = make_float2(j >= 0 && j < a.ck ? load_weight(a.w1, at, a.w_dtype) * a.scale : 0.0f,
+                              j >= 0 && j < a.ck && h + 1 < H ? load_weight(a.w1, at + a.cq * a.ck, a.w_dtype) * a.scale : 0.0f);
     }
     const int quads = tile / 4, oquads = round4(H) / 4;
     int stage = 0, stages = 0;                                   // of the whole run: what is not waited for at its end
@@ -416,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                 barrier_sync(BAR_FULL + (stage & 1), THREADS);
                 // conv: (two heads, row, four keys) a thread
                 const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group, pairs = (heads + 1) / 2;
-                const int q0 = ((k0 - left + turn + shift) % ring.keys) >> 2;
+                const int q0 = ((k0 - left - first_tap + turn + ring.keys) % ring.keys) >> 2;
                 for (int i = tid; i < pairs * a.cq2 << (a.shift - 2); i += ROLE_THREADS) {
                     const int quad = i & (quads - 1), rest = i >> (a.shift - 2), r = rest / pairs, pair = rest - r * pairs;
                     int q1 = q0 + quad;
@@ -555,11 +548,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         };
         enter_span(begin);
         enter_stage();
-        struct Task {
-            int task, unit, stage;
-            bool first, final;     // of its task and stage
-        };
-        auto fetch = [&](V& values, Task& t) -> bool {
+        constexpr int N = TOGETHER<T, DMAX>;
+        V values[N];
+        int t_task = 0, t_unit = 0, t_units = 0;                 // whose values are on their way
+        bool t_first = false;                                    // of its task and stage
+        auto fetch = [&]() -> bool {
             while (!cur.done && (cur.task >= tasks || cur.unit >= cur.last)) {
                 if (cur.task < tasks) {
                     cur.task += ROLE_WARPS;
@@ -576,12 +569,18 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 enter_stage();
             }
             if (cur.done) return false;
-            const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit);
             const int copy = cur.task % copies, hk = cur.task / copies * GT / group;
-            t.task = cur.task; t.unit = cur.unit; t.stage = cur.stage;
-            t.first = cur.unit == copy * (tile / KEYS) / copies;
-            values.load(pool, base < 0 ? base : base + (long)hk * head_stride, cur.s.len - (cur.k0 + cur.unit * KEYS), c.D, lane);
-            t.final = ++cur.unit == cur.last;
+            const long head = (long)hk * head_stride;
+            t_task = cur.task; t_unit = cur.unit;
+            t_first = cur.unit == copy * (tile / KEYS) / copies;
+            t_units = cur.last - cur.unit;                       // N or fewer: the last of the task and stage
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int u = cur.unit + i;
+                const long base = __shfl_sync(0xffffffffu, cur.at, u);
+                if (i == 0 || i < t_units) values[i].load(pool, base < 0 ? base : base + head, cur.s.len - (cur.k0 + u * KEYS), c.D, lane);
+            }
+            cur.unit += N;
             return true;
         };
         int stage = 0, stages = 0;
@@ -630,13 +629,13 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         };
         barrier_sync(BAR_MEMORY, ROLE_THREADS);                  // the outputs are zero
         bool started = false;
-        auto work = [&](V& values, Task& t) -> bool {
+        for (bool more = fetch(); more;) {
+            // the cursor still stands where this task's values were fetched
             if (!started) barrier_sync(BAR_FULL, THREADS);       // the first stage
             started = true;
-            pass_stages(t.stage);
-            const int unit = t.unit, copy = t.task % copies, h0 = t.task / copies * GT;
-            const bool first = t.first, final = t.final;
-            bool more = true;
+            pass_stages(cur.stage);
+            const int unit = t_unit, units = t_units, copy = t_task % copies, h0 = t_task / copies * GT;
+            const bool first = t_first, final = t_units <= N;
             const T* weights = a_sm + (stage & 1) * a_other;
             if (first) {
 #pragma unroll
@@ -648,8 +647,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 const int y = g / P::STRIDE, piece = g % P::STRIDE;
                 const bool on = y < GT && piece < P::PIECES;
                 const uint32_t* col = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4 + unit * 8;
-                values.multiply(acc, on ? col[0] : 0u, on ? col[4] : 0u);
-                more = fetch(values, t);
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i == 0 || i < units) values[i].multiply(acc, on ? col[i * 8] : 0u, on ? col[i * 8 + 4] : 0u);
+                more = fetch();
                 if (final) {
                     // sum over the pieces; a head's columns are those of one lane (four heads) or of two, which then halve the elements
                     const int head = h0 + t4 * 2 / P::STRIDE;
@@ -688,17 +689,21 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < V::STEPS; ++i) {
-                    float f[4];
-                    unpack16<float>(values.r[i], f);
+                for (int n_ = 0; n_ < N; ++n_) {
+                    if (n_ > 0 && n_ >= units) break;
 #pragma unroll
-                    for (int y = 0; y < GT; ++y) {
-                        const float p = weights[((h0 + y) << a.shift) + unit * KEYS + i * V::SUBS + lane / V::ROWLANES];
+                    for (int i = 0; i < V::STEPS; ++i) {
+                        float f[4];
+                        unpack16<float>(values[n_].r[i], f);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[y][0][e] = fmaf(p, f[e], acc[y][0][e]);
+                        for (int y = 0; y < GT; ++y) {
+                            const float p = weights[((h0 + y) << a.shift) + (unit + n_) * KEYS + i * V::SUBS + lane / V::ROWLANES];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[y][0][e] = fmaf(p, f[e], acc[y][0][e]);
+                        }
                     }
                 }
-                more = fetch(values, t);
+                more = fetch();
                 if (final) {
                     const int e0 = (lane % V::ROWLANES) * 4;
 #pragma unroll
@@ -716,9 +721,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                     }
                 }
             }
-            return more;
-        };
-        in_turns<V, Task, TWO_IN_FLIGHT<T, DMAX>>(fetch, work);
+        }
         if (!started) barrier_sync(BAR_FULL, THREADS);           // no task at all
         pass_stages(stages);
         return;
