@@ -127,6 +127,58 @@ __device__ __forceinline__ void conv_row(float (&z)[4], const float* x, const fl
     }
 }
 
+// The first conv of a stage: (two heads, row, four keys) a thread, sixteen packed FMAs for every four taps.  CHUNKS: quads of taps, 0 when
+// there are more than the kernel has registers for; otherwise a tap row's whole window is loaded before its first FMA, so
+// that the loads' latency is waited for once a row.
+template <int CHUNKS> __device__ __forceinline__ void conv_pairs(const float* s, const float2* taps, float* to, const ScoreRing& ring, int q0, int heads, int H, int R,
+                                                                 int cq, int cq2, int ckp, int shift, int tid) {
+    const int quads = 1 << (shift - 2), pairs = (heads + 1) / 2, wrap = ring.keys / 4;
+    for (int i = tid; i < pairs * cq2 * quads; i += ROLE_THREADS) {
+        const int quad = i & (quads - 1), rest = i >> (shift - 2), r = rest / pairs, pair = rest - r * pairs;
+        int at[CHUNKS + 1];
+        at[0] = q0 + quad;
+        if (at[0] >= wrap) at[0] -= wrap;
+#pragma unroll
+        for (int j = 1; j <= CHUNKS; ++j) at[j] = at[j - 1] + 1 == wrap ? 0 : at[j - 1] + 1;
+        float2 z[4];
+        z[0] = z[1] = z[2] = z[3] = make_float2(0.0f, 0.0f);
+        const float* row = s + (pair * R + r) * ring.row;
+        const float4* w = reinterpret_cast<const float4*>(taps + pair * cq * ckp);
+        auto step = [&](const float4& e, const float4& o, const float4& e1, const float4& o1, const float4& wa, const float4& wb) {
+            const float2 v[7] = {make_float2(e.x, e.y), make_float2(e.z, e.w), make_float2(o.x, o.y), make_float2(o.z, o.w),
+                                 make_float2(e1.x, e1.y), make_float2(e1.z, e1.w), make_float2(o1.x, o1.y)};
+            const float2 ws[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[k] = __ffma2_rn(ws[t], v[k + t], z[k]);
+        };
+        for (int tap = 0; tap < cq; ++tap, row += ring.row) {
+            const float4 *e4 = reinterpret_cast<const float4*>(row), *o4 = reinterpret_cast<const float4*>(row + ring.half);
+            if constexpr (CHUNKS > 0) {
+                float4 e[CHUNKS + 1], o[CHUNKS + 1];
+#pragma unroll
+                for (int j = 0; j <= CHUNKS; ++j) { e[j] = e4[at[j]]; o[j] = o4[at[j]]; }
+#pragma unroll
+                for (int j = 0; j < CHUNKS; ++j) step(e[j], o[j], e[j + 1], o[j + 1], w[2 * j], w[2 * j + 1]);
+                w += 2 * CHUNKS;
+            } else {
+                int x = at[0];
+                float4 e = e4[x], o = o4[x];
+                for (int j = 0; j < ckp / 4; ++j, w += 2) {
+                    x = x + 1 == wrap ? 0 : x + 1;
+                    const float4 e1 = e4[x], o1 = o4[x];
+                    step(e, o, e1, o1, w[0], w[1]);
+                    e = e1; o = o1;
+                }
+            }
+        }
+        float* out = to + ((r * H + 2 * pair) << shift) + 4 * quad;
+        *reinterpret_cast<float4*>(out) = make_float4(z[0].x, z[1].x, z[2].x, z[3].x);
+        if (2 * pair + 1 < heads) *reinterpret_cast<float4*>(out + (1 << shift)) = make_float4(z[0].y, z[1].y, z[2].y, z[3].y);
+    }
+}
+
 // z[o][k] = sum_h W[h][o0 + o] from[h][k0 + k] for four heads and four keys.
 __device__ __forceinline__ void mix_heads(float (&z)[4][4], const float* W, const float* from, int H, int tile) {
     const int Hp = round4(H);
@@ -408,36 +460,17 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             for (int hk0 = 0; hk0 < c.kv_heads; hk0 += a.kv_together, ++stage) {
                 barrier_sync(BAR_FULL + (stage & 1), THREADS);
                 // conv: (two heads, row, four keys) a thread
-                const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group, pairs = (heads + 1) / 2;
+                const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group;
                 const int q0 = ((k0 - left - first_tap + turn + ring.keys) % ring.keys) >> 2;
-                for (int i = tid; i < pairs * a.cq2 << (a.shift - 2); i += ROLE_THREADS) {
-                    const int quad = i & (quads - 1), rest = i >> (a.shift - 2), r = rest / pairs, pair = rest - r * pairs;
-                    int q1 = q0 + quad;
-                    if (q1 >= ring.keys / 4) q1 -= ring.keys / 4;
-                    float2 z[4];
-                    z[0] = z[1] = z[2] = z[3] = make_float2(0.0f, 0.0f);
-                    const float* srow = s_sm + (stage & 1) * s_other + (pair * R + r) * ring.row;
-                    const float4* w = reinterpret_cast<const float4*>(t_sm + (hk0 * group / 2 + pair) * a.cq * ckp);
-                    for (int tap = 0; tap < a.cq; ++tap, srow += ring.row) {
-                        const float4 *e4 = reinterpret_cast<const float4*>(srow), *o4 = reinterpret_cast<const float4*>(srow + ring.half);
-                        int at = q1;
-                        float4 e = e4[at], o = o4[at];
-                        for (int j = 0; j < ckp / 4; ++j, w += 2) {
-                            at = at + 1 == ring.keys / 4 ? 0 : at + 1;
-                            const float4 e1 = e4[at], o1 = o4[at], wa = w[0], wb = w[1];
-                            const float2 v[7] = {make_float2(e.x, e.y), make_float2(e.z, e.w), make_float2(o.x, o.y), make_float2(o.z, o.w),
-                                                 make_float2(e1.x, e1.y), make_float2(e1.z, e1.w), make_float2(o1.x, o1.y)};
-                            const float2 ws[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
-#pragma unroll
-                            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) z[k] = __ffma2_rn(ws[t], v[k + t], z[k]);
-                            e = e1; o = o1;
-                        }
-                    }
-                    float* to = c_sm + ((r * H + hk0 * group + 2 * pair) << a.shift) + 4 * quad;
-                    *reinterpret_cast<float4*>(to) = make_float4(z[0].x, z[1].x, z[2].x, z[3].x);
-                    if (2 * pair + 1 < heads) *reinterpret_cast<float4*>(to + tile) = make_float4(z[0].y, z[1].y, z[2].y, z[3].y);
+                const float* s_now = s_sm + (stage & 1) * s_other;
+                const float2* t_now = t_sm + hk0 * group / 2 * a.cq * ckp;
+                float* c_now = c_sm + ((hk0 * group) << a.shift);
+                switch (ckp / 4) {
+                    case 1: conv_pairs<1>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
+                    case 2: conv_pairs<2>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
+                    case 3: conv_pairs<3>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
+                    case 4: conv_pairs<4>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
+                    default: conv_pairs<0>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
                 }
                 if (stage + 2 < stages) barrier_arrive(BAR_EMPTY + (stage & 1), THREADS);
             }
@@ -490,14 +523,14 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
 // Tasks of (GT query heads, share of a tile's keys) belong to one warp each; where heads do not divide evenly among the warps, `copies`
 // warps share one and each keeps an output of its own.
 template <typename T, int DMAX, int GT>
-__global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCache c, MtaArgs a, int copies) {
+__global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCache c, MtaArgs a, int copy_shift) {
     constexpr bool HALF = sizeof(T) == 2;
     using V = std::conditional_t<HALF, ValueTile<T, DMAX>, ValueTileF32<DMAX>>;
     using P = Pieces<GT>;
     extern __shared__ __align__(16) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, ckp = round4(a.ck2), left = (a.ck2 - 1) / 2, pp = prob_pitch(tile, a.ck2);
-    const int quads = tile / 4, oquads = round4(H) / 4, ap = piece_pitch(tile);
+    const int quads = tile / 4, oquads = round4(H) / 4, ap = piece_pitch(tile), copies = 1 << copy_shift;
     const ValueSmem m = value_smem(a.B, H, c.D, tile, a.cq2, a.ck2, copies);
     float *p_sm = reinterpret_cast<float*>(smem + m.p), *y_sm = reinterpret_cast<float*>(smem + m.y), *by = reinterpret_cast<float*>(smem + m.by);
     float *W_sm = reinterpret_cast<float*>(smem + m.W), *t_sm = reinterpret_cast<float*>(smem + m.taps), *o_sm = reinterpret_cast<float*>(smem + m.o);
@@ -523,13 +556,18 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
             Span s;
             long at;
             int k0, units, task, unit, last, stage;
+            long head;         // from kv head 0 to the task's
             Pages next;
             bool done;
         } cur = {};
-        auto share = [&] {                                       // the units of this stage that the task's copy has
-            const int copy = cur.task % copies, all = tile / KEYS;
-            cur.unit = copy * all / copies;
-            cur.last = (copy + 1) * all / copies < cur.units ? (copy + 1) * all / copies : cur.units;
+        // The units of this stage that the task's copy has, and where its kv head lies.  Divisions by the group only where they must be: in
+        // the stream of loads they cost more than the products.
+        auto share = [&] {
+            const int copy = cur.task & (copies - 1), all = tile / KEYS, h = cur.task >> copy_shift;
+            cur.unit = copy * all >> copy_shift;
+            cur.last = (copy + 1) * all >> copy_shift;
+            if (cur.last > cur.units) cur.last = cur.units;
+            cur.head = (long)(group == GT ? h : h * GT / group) * head_stride;
         };
         auto enter_stage = [&] {
             cur.units = ((cur.k0 + tile < cur.s.k1 ? cur.k0 + tile : cur.s.k1) - cur.k0) / KEYS;
@@ -569,10 +607,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 enter_stage();
             }
             if (cur.done) return false;
-            const int copy = cur.task % copies, hk = cur.task / copies * GT / group;
-            const long head = (long)hk * head_stride;
+            const int copy = cur.task & (copies - 1);
+            const long head = cur.head;
             t_task = cur.task; t_unit = cur.unit;
-            t_first = cur.unit == copy * (tile / KEYS) / copies;
+            t_first = cur.unit == copy * (tile / KEYS) >> copy_shift;
             t_units = cur.last - cur.unit;                       // N or fewer: the last of the task and stage
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -634,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
             if (!started) barrier_sync(BAR_FULL, THREADS);       // the first stage
             started = true;
             pass_stages(cur.stage);
-            const int unit = t_unit, units = t_units, copy = t_task % copies, h0 = t_task / copies * GT;
+            const int unit = t_unit, units = t_units, copy = t_task & (copies - 1), h0 = (t_task >> copy_shift) * GT;
             const bool first = t_first, final = t_units <= N;
             const T* weights = a_sm + (stage & 1) * a_other;
             if (first) {
@@ -935,9 +973,9 @@ template <typename T, int DMAX> int launch_dim(const PagedCache& c, const MtaArg
     const int R = a.cq + a.cq2 - 1;
     if (int rc = R <= 8 ? launch_scores<T, DMAX, 1>(c, a, p, st) : R <= 16 ? launch_scores<T, DMAX, 2>(c, a, p, st) : launch_scores<T, DMAX, 4>(c, a, p, st)) return rc;
     int rc = 0;
-    if (p.gt == 4) rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 4>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies);
-    else if (p.gt == 2) rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 2>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies);
-    else rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 1>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies);
+    if (p.gt == 4) rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 4>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies == 4 ? 2 : p.copies - 1);
+    else if (p.gt == 2) rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 2>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies == 4 ? 2 : p.copies - 1);
+    else rc = launch_kernel<mta_decode_values_kernel<T, DMAX, 1>>("mta_decode_values_kernel", dim3(p.workers), THREADS, p.value_bytes, st, c, a, p.copies == 4 ? 2 : p.copies - 1);
     if (rc) return rc;
     return launch_kernel<mta_decode_join_kernel<T>>("mta_decode_join_kernel", dim3(c.H, a.B), 128, (2 * a.B + 1) * sizeof(int), st, c, a);
 }
