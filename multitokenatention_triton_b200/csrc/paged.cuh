@@ -53,6 +53,13 @@ template <> __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 bytes that are read once: past L1, which keeps the queries.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
 // 16 keys of one head in a warp's registers, DMAX >= D elements each.  Lane (g, t) = (lane / 4, lane % 4) holds of rows g and g + 8
 // the 16 bytes at chunk c * 64 + t * 16: whole 16-byte loads, four lanes on 64 contiguous bytes.  An mma sums over its k index in
 // any order, so the elements of a lane's 16 bytes may stand for any k as long as the queries are read the same way.  The keys are the
@@ -197,13 +204,13 @@ template <int DMAX> struct ValueTileF32 {
         if (base >= 0 && live >= KEYS && D == DMAX) {
             const float* row = pool + base + (sub * DMAX + e);
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) r[i] = __ldg(reinterpret_cast<const uint4*>(row + i * SUBS * DMAX));
+            for (int i = 0; i < STEPS; ++i) r[i] = load_once((row + i * SUBS * DMAX));
             return;
         }
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
             r[i] = make_uint4(0, 0, 0, 0);
-            if (base >= 0 && i * SUBS + sub < live && e < D) r[i] = __ldg(reinterpret_cast<const uint4*>(pool + base + (long)(i * SUBS + sub) * D + e));
+            if (base >= 0 && i * SUBS + sub < live && e < D) r[i] = load_once((pool + base + (long)(i * SUBS + sub) * D + e));
         }
     }
 };
@@ -231,7 +238,7 @@ template <typename T, int DMAX> struct ValueTile {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) r[i][c] = __ldg(reinterpret_cast<const uint4*>(row + ((i & 1) + (i >> 1) * 8) * DMAX + c * 64));
+                for (int c = 0; c < CHUNKS; ++c) r[i][c] = load_once((row + ((i & 1) + (i >> 1) * 8) * DMAX + c * 64));
             return;
         }
 #pragma unroll
@@ -243,7 +250,7 @@ template <typename T, int DMAX> struct ValueTile {
             for (int c = 0; c < CHUNKS; ++c) {
                 const int e = c * 64 + g * 8;
                 r[i][c] = make_uint4(0, 0, 0, 0);
-                if (on && e < D) r[i][c] = __ldg(reinterpret_cast<const uint4*>(row + e));
+                if (on && e < D) r[i][c] = load_once((row + e));
             }
         }
     }

@@ -234,7 +234,7 @@ struct Pages {
 
 // Tiles of 16 keys or values that a warp's task has and its registers hold in flight: as many as fit.  One at a time left the memory at
 // 3.4 TB/s, and what a task costs besides its loads and products is paid half as often.
-template <typename T, int DMAX> constexpr int TOGETHER = sizeof(T) * DMAX <= 256 ? 2 : 1;
+template <typename T, int DMAX, int NT = 1> constexpr int TOGETHER = sizeof(T) * DMAX <= 256 && NT <= 2 ? 2 : 1;
 
 // The registers of a block are dealt anew once the roles part: 168 to a thread of the memory half, 88 to one of the other, 128 * 512 in all.
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
         const T* pool = static_cast<const T*>(c.k);
         const T* queries = static_cast<const T*>(c.q_hist);
         const int head_stride = c.D << c.page_shift;
-        constexpr int N = TOGETHER<T, DMAX>;
+        constexpr int N = TOGETHER<T, DMAX, NT>;
         long* q_at = reinterpret_cast<long*>(smem + m.q_at) + warp * DECODE_MAX_ROWS;       // this warp's query rows
         // Where the loads are, one task ahead of the arithmetic.
         struct Cursor {
@@ -310,8 +310,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
         enter_span(begin, 0);
         enter_stage();
         K keys[N];
-        int task_unit = 0, task_hk = 0;                          // whose keys are on their way
-        auto fetch = [&]() -> bool {
+        int task_unit = 0, task_hk = 0;                          // whose keys are on their way or next
+        long next_at[N];                                         // where those lie, -1: nowhere
+        int next_live = 0;
+        // Sets the next task; load(i) then starts the loads of its i-th 16 keys.
+        auto advance = [&]() -> bool {
             while (!cur.done && cur.tasks_left == 0) {
                 ++cur.stage;
                 cur.hk0 += a.kv_together;
@@ -332,35 +335,65 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             const long head = (long)(cur.hk0 + cur.hk) * head_stride;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int u = cur.unit + i;
-                const long base = __shfl_sync(0xffffffffu, cur.at, u);       // -1 behind the last unit
-                keys[i].load(pool, base < 0 ? base : base + head, cur.s.len - (cur.first + u * KEYS), c.D, lane);
+                const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit + i);    // -1 behind the last unit
+                next_at[i] = base < 0 ? base : base + head;
             }
+            next_live = cur.s.len - (cur.first + cur.unit * KEYS);
             cur.unit += N;
             if (cur.unit >= cur.units) { cur.unit = 0; ++cur.hk; }
             --cur.tasks_left;
             return true;
         };
+        auto load = [&](int i) { keys[i].load(pool, next_at[i], next_live - i * KEYS, c.D, lane); };
         int stage = 0, span_b = -1, q_head = -1;
         constexpr int PARTS = K::template PARTS<NT * 8>;
         uint4 q[HALF ? PARTS / 2 : 1][HALF ? 2 * K::CH : 1];     // the A operands of a head
-        // Scores of one task into the ring; the registers of its keys take the next task's as soon as they are free.
-        for (bool more = fetch(); more;) {
-            // the cursor still stands where this task's keys were fetched
+        // The span's query rows, and the queries of one head as A operands.
+        auto query_rows = [&] {
+            if (cur.s.b == span_b) return;
+            __syncwarp();
+            const int pos = cur.s.len - R + lane;
+            q_at[lane] = lane < R && pos >= 0 ? ((long)cur.s.slot * c.ring + pos % c.ring) * H * c.D : -1;
+            span_b = cur.s.b;
+            q_head = -1;
+            __syncwarp();
+        };
+        auto need_queries = [&](int head) {
+            if constexpr (HALF) {
+                if (q_head == head) return;
+                q_head = head;
+                const T* qh = queries + (long)head * c.D;
+#pragma unroll
+                for (int m_ = 0; m_ < PARTS / 2; ++m_) {
+                    const long r0 = q_at[16 * m_ + g], r1 = NT > 1 ? q_at[16 * m_ + 8 + g] : -1;
+#pragma unroll
+                    for (int ch = 0; ch < K::CH; ++ch) {
+                        const int e = (ch * 4 + t4) * K::EPL;
+                        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+                        if (r0 >= 0 && e < c.D) lo = __ldg(reinterpret_cast<const uint4*>(qh + r0 + e));
+                        if (NT > 1 && r1 >= 0 && e < c.D) hi = __ldg(reinterpret_cast<const uint4*>(qh + r1 + e));
+                        q[m_][2 * ch] = make_uint4(lo.x, hi.x, lo.y, hi.y);
+                        q[m_][2 * ch + 1] = make_uint4(lo.z, hi.z, lo.w, hi.w);
+                    }
+                }
+            }
+        };
+        bool more = advance();
+        if (more) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) load(i);
+            query_rows();
+            need_queries((cur.hk0 + task_hk) * group);
+        }
+        // Scores of one task into the ring; the registers of its keys and queries take the next task's as soon as they are free.
+        while (more) {
+            // the cursor still stands where this task's keys lie
             while (stage < cur.stage) {
                 barrier_arrive(BAR_FULL + (stage & 1), THREADS);
                 ++stage;
                 if (stage >= 2) barrier_sync(BAR_EMPTY + (stage & 1), THREADS);
             }
             const int len = cur.s.len;
-            if (cur.s.b != span_b) {
-                __syncwarp();
-                const int pos = len - R + lane;
-                q_at[lane] = lane < R && pos >= 0 ? ((long)cur.s.slot * c.ring + pos % c.ring) * H * c.D : -1;
-                span_b = cur.s.b;
-                q_head = -1;
-                __syncwarp();
-            }
             const int first_key = cur.first + task_unit * KEYS, local = task_hk * group, head0 = (cur.hk0 + task_hk) * group;
             const int units = cur.units - task_unit;                                 // of this task, if less than N
             int place = cur.place + task_unit * KEYS;
@@ -368,37 +401,29 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             const bool full = first_key + N * KEYS - 1 <= len - R;                   // every row sees every key
             float* buf = s_sm + (stage & 1) * s_other;
             for (int gq = 0; gq < group; ++gq) {
-                const T* qh = queries + (long)(head0 + gq) * c.D;
                 float acc[N][PARTS][4];
-                if constexpr (HALF) {
-                    if (q_head != head0 + gq) {
+                need_queries(head0 + gq);
+                const bool last = gq == group - 1;
+                if (last) more = advance();
+                // the loads of the next keys start as soon as their registers are free, one tile after the other
 #pragma unroll
-                        for (int m_ = 0; m_ < PARTS / 2; ++m_) {
-                            const long r0 = q_at[16 * m_ + g], r1 = NT > 1 ? q_at[16 * m_ + 8 + g] : -1;
-#pragma unroll
-                            for (int ch = 0; ch < K::CH; ++ch) {
-                                const int e = (ch * 4 + t4) * K::EPL;
-                                uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-                                if (r0 >= 0 && e < c.D) lo = __ldg(reinterpret_cast<const uint4*>(qh + r0 + e));
-                                if (r1 >= 0 && e < c.D) hi = __ldg(reinterpret_cast<const uint4*>(qh + r1 + e));
-                                q[m_][2 * ch] = make_uint4(lo.x, hi.x, lo.y, hi.y);
-                                q[m_][2 * ch + 1] = make_uint4(lo.z, hi.z, lo.w, hi.w);
-                            }
-                        }
-                        q_head = head0 + gq;
-                    }
-#pragma unroll
-                    for (int i = 0; i < N; ++i) keys[i].template score<NT * 8>(acc[i], lane, [&](int m_, int x) { return q[m_][x]; });
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
+                for (int i = 0; i < N; ++i) {
+                    if constexpr (HALF) {
+                        keys[i].template score<NT * 8>(acc[i], lane, [&](int m_, int x) { return q[m_][x]; });
+                    } else {
+                        const T* qh = queries + (long)(head0 + gq) * c.D;
                         keys[i].template score<NT * 8>(acc[i], lane, [&](int row, int ch) {
                             const long r = q_at[row];
                             const int e = (ch * 4 + t4) * K::EPL;
                             return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
                         });
+                    }
+                    if (last && more) load(i);
                 }
-                if (gq == group - 1) more = fetch();
+                if (last && more) {
+                    query_rows();
+                    need_queries((cur.hk0 + task_hk) * group);
+                }
                 float* s = buf + ((local + gq) >> 1) * R * ring.row + ((local + gq) & 1);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -588,9 +613,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         enter_stage();
         constexpr int N = TOGETHER<T, DMAX>;
         V values[N];
-        int t_task = 0, t_unit = 0, t_units = 0;                 // whose values are on their way
+        int t_task = 0, t_unit = 0, t_units = 0, next_live = 0;  // whose values are on their way or next
+        long next_at[N];
         bool t_first = false;                                    // of its task and stage
-        auto fetch = [&]() -> bool {
+        auto advance = [&]() -> bool {
             while (!cur.done && (cur.task >= tasks || cur.unit >= cur.last)) {
                 if (cur.task < tasks) {
                     cur.task += ROLE_WARPS;
@@ -614,12 +640,15 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
             t_units = cur.last - cur.unit;                       // N or fewer: the last of the task and stage
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int u = cur.unit + i;
-                const long base = __shfl_sync(0xffffffffu, cur.at, u);
-                if (i == 0 || i < t_units) values[i].load(pool, base < 0 ? base : base + head, cur.s.len - (cur.k0 + u * KEYS), c.D, lane);
+                const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit + i);
+                next_at[i] = base < 0 ? base : base + head;
             }
+            next_live = cur.s.len - (cur.k0 + cur.unit * KEYS);
             cur.unit += N;
             return true;
+        };
+        auto load = [&](int i) {
+            if (i == 0 || i < t_units) values[i].load(pool, next_at[i], next_live - i * KEYS, c.D, lane);
         };
         int stage = 0, stages = 0;
         for (long x = begin; x < end;) {
@@ -667,8 +696,13 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
         };
         barrier_sync(BAR_MEMORY, ROLE_THREADS);                  // the outputs are zero
         bool started = false;
-        for (bool more = fetch(); more;) {
-            // the cursor still stands where this task's values were fetched
+        bool more = advance();
+        if (more) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) load(i);
+        }
+        while (more) {
+            // the cursor still stands where this task's values lie
             if (!started) barrier_sync(BAR_FULL, THREADS);       // the first stage
             started = true;
             pass_stages(cur.stage);
@@ -685,10 +719,12 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                 const int y = g / P::STRIDE, piece = g % P::STRIDE;
                 const bool on = y < GT && piece < P::PIECES;
                 const uint32_t* col = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4 + unit * 8;
+                more = advance();
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+                for (int i = 0; i < N; ++i) {
                     if (i == 0 || i < units) values[i].multiply(acc, on ? col[i * 8] : 0u, on ? col[i * 8 + 4] : 0u);
-                more = fetch();
+                    if (more) load(i);
+                }
                 if (final) {
                     // sum over the pieces; a head's columns are those of one lane (four heads) or of two, which then halve the elements
                     const int head = h0 + t4 * 2 / P::STRIDE;
@@ -741,7 +777,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                         }
                     }
                 }
-                more = fetch();
+                more = advance();
+                if (more) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) load(i);
+                }
                 if (final) {
                     const int e0 = (lane % V::ROWLANES) * 4;
 #pragma unroll
