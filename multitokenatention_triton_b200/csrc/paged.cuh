@@ -53,15 +53,20 @@ template <> __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes that are read once: past L1, which keeps the queries.
+// 16 or 32 bytes that are read once: past L1, which keeps the queries.
 __device__ __forceinline__ uint4 load_once(const void* p) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
     return r;
 }
+__device__ __forceinline__ void load_once(const void* p, uint4& a, uint4& b) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+}
+__device__ __forceinline__ bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 // 16 keys of one head in a warp's registers, DMAX >= D elements each.  Lane (g, t) = (lane / 4, lane % 4) holds of rows g and g + 8
-// the 16 bytes at chunk c * 64 + t * 16: whole 16-byte loads, four lanes on 64 contiguous bytes.  An mma sums over its k index in
+// 32 bytes at 128 p + 32 t, as chunks 2p and 2p + 1: one load each, four lanes on a whole line.  An mma sums over its k index in
 // any order, so the elements of a lane's 16 bytes may stand for any k as long as the queries are read the same way.  The keys are the
 // B operand, two neighbouring registers of a load each; as the A operand, whose four registers would come from two loads, every
 // mma cost seven moves, and the scores of 16 keys three times as many instructions.
@@ -74,18 +79,20 @@ template <typename T, int DMAX> struct KeyTile {
     template <int ROWS> static constexpr int PARTS = HALF ? (ROWS + 15) / 16 * 2 : ROWS / 8;
     static __device__ __forceinline__ int row_of(int p, int i, int lane) { return HALF ? p / 2 * 16 + (lane >> 2) + (i >> 1) * 8 : p * 8 + 2 * (lane & 3) + (i & 1); }
     static __device__ __forceinline__ int key_of(int p, int i, int lane) { return HALF ? p % 2 * 8 + 2 * (lane & 3) + (i & 1) : (lane >> 2) + 8 * (i >> 1); }
+    static __device__ __forceinline__ int element(int c, int t) { return (c / 2 * 8 + t * 2 + c % 2) * EPL; }
     uint4 r[2][CH];
 
     // Rows base, base + 1, ... of which `live` exist; the others are zero and not read.  base < 0: none exists.  The usual whole tile
     // takes a path of plain loads: setting the registers to zero first costs as much as everything else here.
     __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        if (base >= 0 && live >= KEYS && D == DMAX) {
-            const T* row = pool + base + (g * DMAX + t * EPL);
+        const T* first = pool + base;
+        if (base >= 0 && live >= KEYS && D == DMAX && aligned32(first)) {
+            const T* row = first + (g * DMAX + t * 2 * EPL);
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int c = 0; c < CH; ++c) r[x][c] = __ldg(reinterpret_cast<const uint4*>(row + x * 8 * DMAX + c * 4 * EPL));
+                for (int c = 0; c < CH; c += 2) load_once(row + x * 8 * DMAX + c * 4 * EPL, r[x][c], r[x][c + 1]);
             return;
         }
 #pragma unroll
@@ -94,9 +101,9 @@ template <typename T, int DMAX> struct KeyTile {
             const T* row = pool + (on ? base + (long)(g + 8 * x) * D : 0);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const int e = (c * 4 + t) * EPL;
+                const int e = element(c, t);
                 r[x][c] = make_uint4(0, 0, 0, 0);
-                if (on && e < D) r[x][c] = __ldg(reinterpret_cast<const uint4*>(row + e));
+                if (on && e < D) r[x][c] = load_once(row + e);
             }
         }
     }
@@ -216,8 +223,8 @@ template <int DMAX> struct ValueTileF32 {
 };
 
 // 16 values of one head in 16 bits as the A operand of mma.sync, transposed: rows are elements, columns keys.  Lane (g, t) loads
-// the 16 bytes at element 64c + 8g of keys 2t, 2t + 1, 2t + 8 and 2t + 9 (8 lanes on 128 contiguous bytes) and pairs neighbouring keys'
-// halves with one byte permute each; mma (c, j) has element 64c + 8g + j as its row g and 64c + 8g + j + 4 as its row g + 8.
+// 32 bytes at 256 p + 32 g, as chunks 2p and 2p + 1 (DMAX 64: 16 bytes at 16 g), of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and pairs neighbouring keys'
+// halves with one byte permute each; mma (c, j) has element e + j as its row g and e + j + 4 as its row g + 8, e = element(c, g).
 //
 // The B operand's eight columns hold the weights of GT heads, each split into PIECES 16-bit numbers that add up to it: columns
 // y * STRIDE + i, i < PIECES, so that an mma that has eight columns anyway multiplies weights of 24 (bf16) or 33 bits (fp16) with the
@@ -229,16 +236,24 @@ template <int GT> struct Pieces {
 };
 template <typename T, int DMAX> struct ValueTile {
     static constexpr int CHUNKS = DMAX / 64;
+    static __device__ __forceinline__ int element(int c, int g) { return CHUNKS == 1 ? g * 8 : c / 2 * 128 + g * 16 + c % 2 * 8; }
     uint4 r[4][CHUNKS];
 
     __device__ __forceinline__ void load(const T* pool, long base, int live, int D, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        if (base >= 0 && live >= KEYS && D == DMAX) {
-            const T* row = pool + base + (2 * t * DMAX + g * 8);
+        const T* first = pool + base;
+        if (base >= 0 && live >= KEYS && D == DMAX && aligned32(first)) {
+            const T* row = first + 2 * t * DMAX + element(0, g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                const T* at = row + ((i & 1) + (i >> 1) * 8) * DMAX;
+                if constexpr (CHUNKS == 1) {
+                    r[i][0] = load_once(at);
+                } else {
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) r[i][c] = load_once((row + ((i & 1) + (i >> 1) * 8) * DMAX + c * 64));
+                    for (int c = 0; c < CHUNKS; c += 2) load_once(at + c * 64, r[i][c], r[i][c + 1]);
+                }
+            }
             return;
         }
 #pragma unroll
@@ -248,13 +263,13 @@ template <typename T, int DMAX> struct ValueTile {
             const T* row = pool + (on ? base + (long)key * D : 0);
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
-                const int e = c * 64 + g * 8;
+                const int e = element(c, g);
                 r[i][c] = make_uint4(0, 0, 0, 0);
                 if (on && e < D) r[i][c] = load_once((row + e));
             }
         }
     }
-    // acc[c][j] += values x weights: [0], [1] element 64c + 8g + j, columns 2t and 2t + 1; [2], [3] element 64c + 8g + j + 4.
+    // acc[c][j] += values x weights: [0], [1] element(c, g) + j, columns 2t and 2t + 1; [2], [3] element(c, g) + j + 4.
     __device__ __forceinline__ void multiply(float (&acc)[CHUNKS][4][4], uint32_t b0, uint32_t b1) const {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {

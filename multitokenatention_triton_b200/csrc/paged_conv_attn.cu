@@ -110,13 +110,14 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
 
         // queries and taps of this line
         for (int i = lane; i < QROWS * (DMAX / EPL); i += 32) {
-            const int row = i / (DMAX / EPL), e = (i % (DMAX / EPL)) * EPL, gq = row / (2 * cqp), tap = row % (2 * cqp), pos = len - a.cq + tap;
+            const int row = i / (DMAX / EPL), piece = i % (DMAX / EPL), e = piece * EPL, gq = row / (2 * cqp), tap = row % (2 * cqp), pos = len - a.cq + tap;
             uint4 u = make_uint4(0, 0, 0, 0);
             if (gq < GT && tap < a.cq && pos >= 0 && e < c.D)
                 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(c.q_hist) + (((long)slot * c.ring + pos % c.ring) * c.H + h0 + gq) * c.D + e);
             if constexpr (HALF) {
                 // 16 bytes of a row: the first two registers of one half of the chunk, then of the other, for lane (row % 8, position)
-                uint32_t* to = reinterpret_cast<uint32_t*>(q_sm + ((row / 16 * K::CH + e / 32) * 2 * 32 + row % 8 * 4 + e / 8 % 4) * 16) + row / 8 % 2;
+                // 16 bytes number `piece` of a row are chunk 2p + piece % 2, p = piece / 8, of position piece / 2 % 4
+                uint32_t* to = reinterpret_cast<uint32_t*>(q_sm + ((row / 16 * K::CH + piece / 8 * 2 + piece % 2) * 2 * 32 + row % 8 * 4 + piece / 2 % 4) * 16) + row / 8 % 2;
                 to[0] = u.x; to[2] = u.y; to[128] = u.z; to[130] = u.w;
             } else {
                 *reinterpret_cast<uint4*>(q_sm + row * QP + e * (int)sizeof(T)) = u;
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
             float acc[PARTS][4];
             keys.template score<NT * 8>(acc, lane, [&](int row, int ch) {
                 if constexpr (HALF) return reinterpret_cast<const uint4*>(q_sm)[(row * 2 * K::CH + ch) * 32 + lane];
-                else return *reinterpret_cast<const uint4*>(q_sm + row * QP + ch * 64 + t4 * 16);
+                else return *reinterpret_cast<const uint4*>(q_sm + row * QP + K::element(ch, t4) * 4);
             });
             if (u < u1) keys.load(k_pool, key_base(u + 1), live(u + 1), c.D, lane);
             const int col = ((u + 3) % 3) * KEYS + shift;
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] += __shfl_xor_sync(0xffffffffu, f[e], 1);
                 }
-                const int e0 = i * 64 + g * 8;
+                const int e0 = V::element(i, g);
 #pragma unroll
                 for (int y = 0; y < GT; ++y)
                     if (t4 == y * P::STRIDE / 2 && e0 < c.D) store(y, e0, f);

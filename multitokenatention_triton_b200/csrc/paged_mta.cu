@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                     const long r0 = q_at[16 * m_ + g], r1 = NT > 1 ? q_at[16 * m_ + 8 + g] : -1;
 #pragma unroll
                     for (int ch = 0; ch < K::CH; ++ch) {
-                        const int e = (ch * 4 + t4) * K::EPL;
+                        const int e = K::element(ch, t4);
                         uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
                         if (r0 >= 0 && e < c.D) lo = __ldg(reinterpret_cast<const uint4*>(qh + r0 + e));
                         if (NT > 1 && r1 >= 0 && e < c.D) hi = __ldg(reinterpret_cast<const uint4*>(qh + r1 + e));
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                         const T* qh = queries + (long)(head0 + gq) * c.D;
                         keys[i].template score<NT * 8>(acc[i], lane, [&](int row, int ch) {
                             const long r = q_at[row];
-                            const int e = (ch * 4 + t4) * K::EPL;
+                            const int e = K::element(ch, t4);
                             return r >= 0 && e < c.D ? *reinterpret_cast<const uint4*>(qh + r + e) : make_uint4(0, 0, 0, 0);
                         });
                     }
@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                         float f[8];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) { f[j] = acc[i][j][0] + acc[i][j][1]; f[j + 4] = acc[i][j][2] + acc[i][j][3]; }
-                        const int e0 = i * 64 + g * 8;
+                        const int e0 = V::element(i, g);
                         if constexpr (P::STRIDE == 4) {
                             float h[4];
 #pragma unroll
