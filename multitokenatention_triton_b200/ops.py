@@ -362,39 +362,59 @@ def host_pipeline_release(device: Optional[torch.device] = None) -> None:
         check(lib().mta_host_pipeline_release(), "mta_host_pipeline_release")
 
 
+# A decoding step is a few launches of a few microseconds: the checks of the calls below read each property of a tensor once.
 def _cache_sizes(what: str, q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                 slots: Optional[torch.Tensor]) -> Tuple[int, ...]:
-    """Checks the tensors of a cache and returns (slots, table width, pages, page size, ring, heads, kv heads, head dim)."""
-    if q_hist.dim() != 4 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape or table.dim() != 2 or lengths.shape != table.shape[:1]:
+                 slots: Optional[torch.Tensor]) -> Tuple[int, Tuple[int, ...]]:
+    """Checks the tensors of a cache and returns (device index, (slots, table width, pages, page size, ring, heads, kv heads, head dim))."""
+    q_shape, k_shape, t_shape = q_hist.shape, k_pages.shape, table.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or v_pages.shape != k_shape or len(t_shape) != 2 or lengths.shape != t_shape[:1]:
         raise MTALibraryError(f"{what}: expected q_hist (slots,ring,H,D), k_pages and v_pages (pages,kv heads,page,D), table (slots,width) and lengths "
-                              f"(slots,), got {tuple(q_hist.shape)}, {tuple(k_pages.shape)}, {tuple(v_pages.shape)}, {tuple(table.shape)}, {tuple(lengths.shape)}")
-    n, ring, H, D = q_hist.shape
-    pages, kv_heads, page, d = k_pages.shape
-    if d != D or table.shape[0] != n or k_pages.dtype != q_hist.dtype or v_pages.dtype != q_hist.dtype:
-        raise MTALibraryError(f"{what}: queries {tuple(q_hist.shape)} {q_hist.dtype}, pages {tuple(k_pages.shape)} {k_pages.dtype} / {v_pages.dtype} and a table "
-                              f"of {table.shape[0]} rows do not belong together")
-    for t in (table, lengths) if slots is None else (table, lengths, slots):
-        if t.dtype != torch.int32:
-            raise MTALibraryError(f"{what}: table, lengths, slots and counts are int32 tensors, got {t.dtype}")
-    dev = q_hist.device
+                              f"(slots,), got {tuple(q_shape)}, {tuple(k_shape)}, {tuple(v_pages.shape)}, {tuple(t_shape)}, {tuple(lengths.shape)}")
+    n, ring, H, D = q_shape
+    pages, kv_heads, page, d = k_shape
+    dtype = q_hist.dtype
+    if d != D or t_shape[0] != n or k_pages.dtype is not dtype or v_pages.dtype is not dtype:
+        raise MTALibraryError(f"{what}: queries {tuple(q_shape)} {dtype}, pages {tuple(k_shape)} {k_pages.dtype} / {v_pages.dtype} and a table of {t_shape[0]} "
+                              "rows do not belong together")
+    i32 = torch.int32
+    if table.dtype is not i32 or lengths.dtype is not i32 or (slots is not None and slots.dtype is not i32):
+        raise MTALibraryError(f"{what}: table, lengths, slots and counts are int32 tensors, got {table.dtype}, {lengths.dtype}"
+                              f"{'' if slots is None else f', {slots.dtype}'}")
+    dev = q_hist.get_device()
     for t in (q_hist, k_pages, v_pages, table, lengths) if slots is None else (q_hist, k_pages, v_pages, table, lengths, slots):
-        if not t.is_cuda or t.device != dev or not t.is_contiguous():
+        if t.get_device() != dev or dev < 0 or not t.is_contiguous():
             raise MTALibraryError(f"{what}: the cache's tensors are contiguous and on one CUDA device, got one on {t.device}"
                                   f"{'' if t.is_contiguous() else ' that is not contiguous'}")
     if slots is not None and slots.dim() != 1:
         raise MTALibraryError(f"{what}: slots has one entry per batch row, got {tuple(slots.shape)}")
-    return n, table.shape[1], pages, page, ring, H, kv_heads, D
+    return dev, (n, t_shape[1], pages, page, ring, H, kv_heads, D)
+
+
+def _launch(dev: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of a device."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, stream_ptr(_DEVICES[dev]))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream_ptr(_DEVICES[dev]))
+    if rc:
+        check(rc, what)
+
+
+_DEVICES = [torch.device("cuda", i) for i in range(64)]
 
 
 _STRIDES9 = ctypes.c_longlong * 9
 
 
-def _token_rows(t: torch.Tensor) -> torch.Tensor:
-    """t as it is where its rows can be read in 16-byte loads, else a contiguous copy."""
+def _token_rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
+    """t as it is where its rows can be read in 16-byte loads, else a contiguous copy; and its strides."""
     e = t.element_size()
     s = t.stride()
-    ok = s[3] == 1 and not (s[0] * e & 15 or s[1] * e & 15 or s[2] * e & 15 or t.data_ptr() & 15)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if s[3] == 1 and not ((s[0] | s[1] | s[2]) * e & 15 or t.data_ptr() & 15):
+        return t, s
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_hist: torch.Tensor,
@@ -402,24 +422,23 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, q: torch.Tensor, k_pages: tor
     """Writes new tokens into a paged cache: k, v (B,kv heads,T,D), q (B,H,T,D), any strides.  Batch row b is slot slots[b] (b when None, no
     slot twice); its counts[b] <= T tokens (T when None) become the last of lengths[slot], which counts them already.  Of its
     queries the last `ring` are kept."""
-    sizes = _cache_sizes("cache_append", q_hist, k_pages, v_pages, table, lengths, slots)
-    n, _, _, _, _, H, kv_heads, D = sizes
-    B, T = (k.shape[0], k.shape[2]) if k.dim() == 4 else (0, 0)
-    if k.shape != (B, kv_heads, T, D) or v.shape != k.shape or q.shape != (B, H, T, D) or not k.dtype == v.dtype == q.dtype == q_hist.dtype:
-        raise MTALibraryError(f"cache_append: expected k, v (B,{kv_heads},T,{D}) and q (B,{H},T,{D}) in {q_hist.dtype}, got {tuple(k.shape)} {k.dtype}, "
-                              f"{tuple(v.shape)} {v.dtype}, {tuple(q.shape)} {q.dtype}")
-    if not k.device == v.device == q.device == q_hist.device:
+    dev, sizes = _cache_sizes("cache_append", q_hist, k_pages, v_pages, table, lengths, slots)
+    _, _, _, _, _, H, kv_heads, D = sizes
+    k_shape, q_shape, dtype = k.shape, q.shape, q_hist.dtype
+    B, T = (k_shape[0], k_shape[2]) if len(k_shape) == 4 else (0, 0)
+    if k_shape != (B, kv_heads, T, D) or v.shape != k_shape or q_shape != (B, H, T, D) or not k.dtype is v.dtype is q.dtype is dtype:
+        raise MTALibraryError(f"cache_append: expected k, v (B,{kv_heads},T,{D}) and q (B,{H},T,{D}) in {dtype}, got {tuple(k_shape)} {k.dtype}, "
+                              f"{tuple(v.shape)} {v.dtype}, {tuple(q_shape)} {q.dtype}")
+    if not k.get_device() == v.get_device() == q.get_device() == dev:
         raise MTALibraryError(f"cache_append: k, v and q must be on the cache's device {q_hist.device}")
     if slots is not None and slots.shape[0] != B:
         raise MTALibraryError(f"cache_append: {slots.shape[0]} slots for {B} batch rows")
-    if counts is not None and (counts.shape != (B,) or counts.dtype != torch.int32 or counts.device != q_hist.device or not counts.is_contiguous()):
+    if counts is not None and (counts.shape != (B,) or counts.dtype is not torch.int32 or counts.get_device() != dev or not counts.is_contiguous()):
         raise MTALibraryError(f"cache_append: counts is a contiguous int32 tensor of {B} entries on {q_hist.device}")
-    k, v, q = _token_rows(k), _token_rows(v), _token_rows(q)
-    strides = _STRIDES9(*k.stride()[:3], *v.stride()[:3], *q.stride()[:3])
-    with on_device(q_hist.device):
-        check(lib().mta_cache_append(k.data_ptr(), v.data_ptr(), q.data_ptr(), strides, None if counts is None else counts.data_ptr(), k_pages.data_ptr(),
-                                     v_pages.data_ptr(), q_hist.data_ptr(), table.data_ptr(), lengths.data_ptr(), None if slots is None else slots.data_ptr(),
-                                     B, T, *sizes, dtype_code(q_hist), stream_ptr(q_hist.device)), "mta_cache_append")
+    (k, ks), (v, vs), (q, qs) = _token_rows(k), _token_rows(v), _token_rows(q)
+    _launch(dev, "mta_cache_append", lib().mta_cache_append, k.data_ptr(), v.data_ptr(), q.data_ptr(), _STRIDES9(*ks[:3], *vs[:3], *qs[:3]),
+            None if counts is None else counts.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q_hist.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            None if slots is None else slots.data_ptr(), B, T, *sizes, dtype_code(q_hist))
 
 
 def cache_copy(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, q_hist: Optional[torch.Tensor] = None,
@@ -446,25 +465,39 @@ def cache_copy(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     if q_hist is not None:
         n_slots, slots = slot_src.shape[0], q_hist.shape[-4]
         slot_elems = q_hist.shape[-3] * q_hist.shape[-2] * q_hist.shape[-1]
-    with on_device(k_pages.device):
-        check(lib().mta_cache_copy(k_pages.data_ptr(), v_pages.data_ptr(), src.data_ptr(), dst.data_ptr(), src.shape[0], page_elems * k_pages.element_size(), pages,
-                                   None if q_hist is None else q_hist.data_ptr(), None if n_slots == 0 else slot_src.data_ptr(),
-                                   None if n_slots == 0 else slot_dst.data_ptr(), n_slots, 0 if q_hist is None else slot_elems * q_hist.element_size(), slots, layers,
-                                   stream_ptr(k_pages.device)), "mta_cache_copy")
+    _launch(k_pages.get_device(), "mta_cache_copy", lib().mta_cache_copy, k_pages.data_ptr(), v_pages.data_ptr(), src.data_ptr(), dst.data_ptr(), src.shape[0],
+            page_elems * k_pages.element_size(), pages, None if q_hist is None else q_hist.data_ptr(), None if n_slots == 0 else slot_src.data_ptr(),
+            None if n_slots == 0 else slot_dst.data_ptr(), n_slots, 0 if q_hist is None else slot_elems * q_hist.element_size(), slots, layers)
 
 
-def _decode_buffers(what: str, q_hist, B, out, workspace, nbytes):
-    """The result (B,H,1,D) and `nbytes` of scratch, the caller's where given."""
-    H, D = q_hist.shape[2:]
+def _decode_weights(q_hist: torch.Tensor, dev: int, *weights: torch.Tensor):
+    """The weights as the library takes them; as they are where they are so already."""
+    dtype = weights[0].dtype
+    if dtype is q_hist.dtype or dtype is torch.float32:
+        for w in weights:
+            if w.dtype is not dtype or w.get_device() != dev or not w.is_contiguous():
+                break
+        else:
+            return weights
+    for w in weights:
+        if w.get_device() != dev:
+            raise MTALibraryError(f"the weights must be on the cache's device {q_hist.device}, got one on {w.device}")
+    if len(weights) == 4:
+        return _mta_weights(q_hist, *weights)
+    return [_weight(w, q_hist, "weight") for w in weights]
+
+
+def _decode_buffers(what, q_hist, B, H, D, dev, out, workspace, nbytes):
+    """The result (B,H,1,D) and scratch, the caller's where given; and the scratch's bytes."""
     if out is None:
-        out = torch.empty(B, H, 1, D, dtype=q_hist.dtype, device=q_hist.device)
-    elif out.shape != (B, H, 1, D) or out.dtype != q_hist.dtype or out.device != q_hist.device or not out.is_contiguous():
+        out = torch.empty((B, H, 1, D), dtype=q_hist.dtype, device=q_hist.device)
+    elif out.shape != (B, H, 1, D) or out.dtype is not q_hist.dtype or out.get_device() != dev or not out.is_contiguous():
         raise MTALibraryError(f"{what}: out must be a contiguous ({B},{H},1,{D}) tensor of {q_hist.dtype} on {q_hist.device}")
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q_hist.device)
-    elif workspace.device != q_hist.device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
+        return out, torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q_hist.device), nbytes
+    if workspace.get_device() != dev or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
         raise MTALibraryError(f"{what}: workspace must be a contiguous tensor of at least {nbytes} bytes on {q_hist.device}")
-    return out, workspace
+    return out, workspace, workspace.numel() * workspace.element_size()
 
 
 def mta_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, w1: torch.Tensor,
@@ -472,23 +505,21 @@ def mta_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The causal MTA forward for the newest token of every sequence of a paged cache: (B,H,1,D).  Batch row b is slot slots[b] (b when
     None); no sequence is longer than max_length; an empty one gets zeros.  Reads the last cq + cq2 - 1 queries of q_hist."""
-    sizes = _cache_sizes("mta_decode", q_hist, k_pages, v_pages, table, lengths, slots)
+    dev, sizes = _cache_sizes("mta_decode", q_hist, k_pages, v_pages, table, lengths, slots)
     B = sizes[0] if slots is None else slots.shape[0]
-    w1, W1, w2, W2 = _mta_weights(q_hist, w1, W1, w2, W2)
-    H, D, kv_heads = sizes[5], sizes[7], sizes[6]
-    if w1.dim() != 3 or w2.dim() != 3 or w1.shape[0] != H or w2.shape[0] != H or W1.shape != (H, H) or W2.shape != (H, H):
-        raise MTALibraryError(f"mta_decode: expected conv weights ({H},cq,ck) and head mixes ({H},{H}), got {tuple(w1.shape)}, {tuple(W1.shape)}, "
-                              f"{tuple(w2.shape)}, {tuple(W2.shape)}")
-    taps = (*w1.shape[1:], *w2.shape[1:])
-    max_length = int(max_length)
-    # zero bytes: a shape that the call refuses below, with the reason
-    nbytes = _size("mta_decode_workspace_bytes", B, H, kv_heads, D, *taps, max_length) if kv_heads and D >= 8 else 0
-    out, workspace = _decode_buffers("mta_decode", q_hist, B, out, workspace, nbytes)
-    with on_device(q_hist.device):
-        check(lib().mta_decode_fwd(q_hist.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                                   None if slots is None else slots.data_ptr(), w1.data_ptr(), W1.data_ptr(), w2.data_ptr(), W2.data_ptr(), out.data_ptr(),
-                                   workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, *sizes, *taps, max_length, dtype_code(q_hist),
-                                   dtype_code(w1), stream_ptr(q_hist.device)), "mta_decode_fwd")
+    H, kv_heads, D = sizes[5:]
+    w1, W1, w2, W2 = _decode_weights(q_hist, dev, w1, W1, w2, W2)
+    s1, s2 = w1.shape, w2.shape
+    if len(s1) != 3 or len(s2) != 3 or s1[0] != H or s2[0] != H or W1.shape != (H, H) or W2.shape != (H, H):
+        raise MTALibraryError(f"mta_decode: expected conv weights ({H},cq,ck) and head mixes ({H},{H}), got {tuple(s1)}, {tuple(W1.shape)}, {tuple(s2)}, "
+                              f"{tuple(W2.shape)}")
+    taps = (s1[1], s1[2], s2[1], s2[2])
+    # zero bytes: a shape that the call refuses, with the reason
+    nbytes = _size("mta_decode_workspace_bytes", B, H, kv_heads, D, *taps, max_length)
+    out, workspace, nbytes = _decode_buffers("mta_decode", q_hist, B, H, D, dev, out, workspace, nbytes)
+    _launch(dev, "mta_decode_fwd", lib().mta_decode_fwd, q_hist.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            None if slots is None else slots.data_ptr(), w1.data_ptr(), W1.data_ptr(), w2.data_ptr(), W2.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes,
+            B, *sizes, *taps, max_length, dtype_code(q_hist), dtype_code(w1))
     return out
 
 
@@ -497,20 +528,18 @@ def conv_attn_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: t
                          out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * conv(Q K^T)) V for the newest token of every sequence of a paged cache: (B,H,1,D); weight (H,cq,ck).  Arguments as in
     mta_decode_fwd; reads the last cq queries of q_hist."""
-    sizes = _cache_sizes("conv_attn_decode", q_hist, k_pages, v_pages, table, lengths, slots)
+    dev, sizes = _cache_sizes("conv_attn_decode", q_hist, k_pages, v_pages, table, lengths, slots)
     B = sizes[0] if slots is None else slots.shape[0]
-    w = _weight(weight, q_hist, "weight")
-    H, D, kv_heads = sizes[5], sizes[7], sizes[6]
-    if w.dim() != 3 or w.shape[0] != H:
-        raise MTALibraryError(f"conv_attn_decode: expected a weight ({H},cq,ck), got {tuple(w.shape)}")
+    H, kv_heads, D = sizes[5:]
+    w, = _decode_weights(q_hist, dev, weight)
+    shape = w.shape
+    if len(shape) != 3 or shape[0] != H:
+        raise MTALibraryError(f"conv_attn_decode: expected a weight ({H},cq,ck), got {tuple(shape)}")
     if softmax_scale is None:
         softmax_scale = 1.0 / (D ** 0.5)
-    max_length = int(max_length)
-    nbytes = _size("mta_conv_attn_decode_workspace_bytes", B, H, kv_heads, D, *w.shape[1:], max_length) if kv_heads and D >= 8 else 0
-    out, workspace = _decode_buffers("conv_attn_decode", q_hist, B, out, workspace, nbytes)
-    with on_device(q_hist.device):
-        check(lib().mta_conv_attn_decode_fwd(q_hist.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                                             None if slots is None else slots.data_ptr(), w.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                                             workspace.numel() * workspace.element_size(), B, *sizes, *w.shape[1:], max_length, float(softmax_scale),
-                                             dtype_code(q_hist), dtype_code(w), stream_ptr(q_hist.device)), "mta_conv_attn_decode_fwd")
+    nbytes = _size("mta_conv_attn_decode_workspace_bytes", B, H, kv_heads, D, shape[1], shape[2], max_length)
+    out, workspace, nbytes = _decode_buffers("conv_attn_decode", q_hist, B, H, D, dev, out, workspace, nbytes)
+    _launch(dev, "mta_conv_attn_decode_fwd", lib().mta_conv_attn_decode_fwd, q_hist.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),
+            lengths.data_ptr(), None if slots is None else slots.data_ptr(), w.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes, B, *sizes, shape[1],
+            shape[2], max_length, softmax_scale, dtype_code(q_hist), dtype_code(w))
     return out
