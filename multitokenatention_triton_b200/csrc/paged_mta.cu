@@ -52,6 +52,8 @@ __host__ __device__ inline int halo(int x) { return (x + KEYS - 1) / KEYS * KEYS
 // Windows begin on multiples of four keys: taps have up to three zeros in front (`lead`) for that, and zeros behind up to `taps`.
 __host__ __device__ inline int lead(int ck) { return (4 - (ck - 1) / 2 % 4) % 4; }
 __host__ __device__ inline int score_taps(int ck) { return round4(ck + lead(ck)); }
+// From one pair of heads' taps to the next pair's: 16 bytes more than they take, so that pairs lie in different banks.
+__host__ __device__ inline int pair_taps(int cq, int ck) { return cq * score_taps(ck) + 2; }
 struct ScoreRing {
     int keys, half, row;   // floats of half a row and of a row
     __host__ __device__ ScoreRing(int tile, int ck, bool whole) {
@@ -74,7 +76,7 @@ __host__ __device__ inline ScoreSmem score_smem(int B, int H, int group, int kv_
     m.s = at; at += m.s_one * (whole ? 1 : 2);
     m.c = at; at += (size_t)cq2 * H * tile * 4;
     m.W = at; at += (size_t)H * round4(H) * 4;
-    m.taps = at; at += (size_t)((H + 1) / 2) * cq * score_taps(ck) * 8;
+    m.taps = at; at += (size_t)((H + 1) / 2) * pair_taps(cq, ck) * 8;
     m.ml = at; at += (size_t)cq2 * H * (tile / 4) * 8;
     m.q_at = at; at += (size_t)ROLE_WARPS * DECODE_MAX_ROWS * 8;
     m.before = at; at += (size_t)(2 * B + 1) * 4;
@@ -143,7 +145,7 @@ template <int CHUNKS> __device__ __forceinline__ void conv_pairs(const float* s,
         float2 z[4];
         z[0] = z[1] = z[2] = z[3] = make_float2(0.0f, 0.0f);
         const float* row = s + (pair * R + r) * ring.row;
-        const float4* w = reinterpret_cast<const float4*>(taps + pair * cq * ckp);
+        const float4* w = reinterpret_cast<const float4*>(taps + pair * (cq * ckp + 2));
         auto step = [&](const float4& e, const float4& o, const float4& e1, const float4& o1, const float4& wa, const float4& wb) {
             const float2 v[7] = {make_float2(e.x, e.y), make_float2(e.z, e.w), make_float2(o.x, o.y), make_float2(o.z, o.w),
                                  make_float2(e1.x, e1.y), make_float2(e1.z, e1.w), make_float2(o1.x, o1.y)};
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     for (int i = tid; i < (H + 1) / 2 * a.cq * ckp; i += ROLE_THREADS) {
         const int j = i % ckp - first_tap, row = i / ckp, tap = row % a.cq, h = row / a.cq * 2;
         const long at = ((long)h * a.cq + tap) * a.ck + j;
-        t_sm[i] = make_float2(j >= 0 && j < a.ck ? load_weight(a.w1, at, a.w_dtype) * a.scale : 0.0f,
+        t_sm[i + h] = make_float2(j >= 0 && j < a.ck ? load_weight(a.w1, at, a.w_dtype) * a.scale : 0.0f,
                               j >= 0 && j < a.ck && h + 1 < H ? load_weight(a.w1, at + a.cq * a.ck, a.w_dtype) * a.scale : 0.0f);
     }
     const int quads = tile / 4, oquads = round4(H) / 4;
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
                 const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group;
                 const int q0 = ((k0 - left - first_tap + turn + ring.keys) % ring.keys) >> 2;
                 const float* s_now = s_sm + (stage & 1) * s_other;
-                const float2* t_now = t_sm + hk0 * group / 2 * a.cq * ckp;
+                const float2* t_now = t_sm + hk0 * group / 2 * pair_taps(a.cq, a.ck);
                 float* c_now = c_sm + ((hk0 * group) << a.shift);
                 switch (ckp / 4) {
                     case 1: conv_pairs<1>(s_now, t_now, c_now, ring, q0, heads, H, R, a.cq, a.cq2, ckp, a.shift, tid); break;
