@@ -293,23 +293,12 @@ template <typename T, int PIECES> __device__ __forceinline__ void split_pieces(f
     }
 }
 
-// Maximum over the warp in one instruction.
-__device__ __forceinline__ float warp_max(float x) {
-    float y;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-    return y;
-}
 // 2^x to a relative 2^-22; 0 below the smallest normal number.
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Brings memory into L2 ahead of its use: 16-byte aligned, a multiple of 16 bytes.
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
 // Work on sequences of different lengths is cut into `workers` equal runs of tiles; a run may begin in one sequence (line) and end
 // in another.  Tile range of worker w of n tiles, and the worker that has tile x.
 __device__ __forceinline__ long run_begin(long w, long n, long workers) { return w * n / workers; }

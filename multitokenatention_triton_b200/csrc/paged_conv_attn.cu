@@ -57,11 +57,10 @@ template <typename T, int DMAX, int GT, int NT> __host__ __device__ constexpr si
            (sizeof(T) == 2 ? 8 * P_PITCH * 2 : GT * KEYS * 4);
 }
 
-// Two neighbouring keys of the conv, summed over the pairs of tap rows i, i + 4, ... of lane group i = lane / 8: .x the first rows of
-// the pairs, .y the second.  `first`: where the window begins in the ring, in units of two keys.  QUADS: taps / 4, 0: not known.
-template <int QUADS> __device__ __forceinline__ void conv_row_pairs(float2& z0, float2& z1, const float* rows, const float* taps, int first, int cqp, int ckp, int lane) {
+// Two neighbouring keys of the conv, summed over the pairs of tap rows i, i + every, ...: .x the first rows of the pairs, .y the second.  `first`: where the window begins in the ring, in units of two keys.  QUADS: taps / 4, 0: not known.
+template <int QUADS> __device__ __forceinline__ void conv_row_pairs(float2& z0, float2& z1, const float* rows, const float* taps, int first, int i, int every, int cqp, int ckp) {
     const int steps = QUADS ? 2 * QUADS : ckp / 2;
-    for (int i = lane >> 3; i < cqp; i += 4) {
+    for (; i < cqp; i += every) {
         const float4 *srow = reinterpret_cast<const float4*>(rows + i * RING_PITCH), *wrow = reinterpret_cast<const float4*>(taps + i * (ckp + 2) * 2);
         int at = first;
         float4 lo = srow[at];
@@ -160,10 +159,11 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
         }
         __syncwarp();
 
-        float m[GT], l[GT];                                          // l: this lane's own keys
+        // lane (head, share of the tap rows, pair of keys): maximum of its head, sum of its own keys
+        constexpr int SHARES = 4 / GT;
+        const int my_head = lane / (8 * SHARES), share = (lane >> 3) % SHARES, pair = lane & 7;
+        float m = -INFINITY, l = 0.0f;
         float o[HALF ? DMAX / 64 : GT][4][4];                        // mma accumulators; float32: [head][0][element]
-#pragma unroll
-        for (int y = 0; y < GT; ++y) { m[y] = -INFINITY; l[y] = 0.0f; }
 #pragma unroll
         for (int i = 0; i < (HALF ? DMAX / 64 : GT); ++i)
 #pragma unroll
@@ -205,75 +205,67 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
             __syncwarp();
             if (u > u0) {
                 const int un = u - 1;
-                // conv: lane (i, pair of keys) sums the pairs of tap rows i, i + 4, ...; then the four lanes of a key are added
-                int first = (un % 3) * KEYS + 2 * (lane & 7) + shift - left;       // even
+                int first = (un % 3) * KEYS + 2 * pair + shift - left;             // even
                 if (first < 0) first += RING;
-                float fade[GT];
-                bool moved = false;
+                float2 z0 = make_float2(0.0f, 0.0f), z1 = z0;
+                const float *rows = s_sm + my_head * cqp * RING_PITCH, *taps = reinterpret_cast<const float*>(w_sm + my_head * cqp * taps_pitch(a.ck));
+                switch (ckp / 4) {
+                    case 1: conv_row_pairs<1>(z0, z1, rows, taps, first / 2, share, SHARES, cqp, ckp); break;
+                    case 2: conv_row_pairs<2>(z0, z1, rows, taps, first / 2, share, SHARES, cqp, ckp); break;
+                    case 3: conv_row_pairs<3>(z0, z1, rows, taps, first / 2, share, SHARES, cqp, ckp); break;
+                    case 4: conv_row_pairs<4>(z0, z1, rows, taps, first / 2, share, SHARES, cqp, ckp); break;
+                    default: conv_row_pairs<0>(z0, z1, rows, taps, first / 2, share, SHARES, cqp, ckp); break;
+                }
+                float z[2] = {z0.x + z0.y, z1.x + z1.y}, p[2];
 #pragma unroll
-                for (int y = 0; y < GT; ++y) {
-                    float2 z0 = make_float2(0.0f, 0.0f), z1 = z0;
-                    const float *rows = s_sm + y * cqp * RING_PITCH, *taps = reinterpret_cast<const float*>(w_sm + y * cqp * taps_pitch(a.ck));
-                    switch (ckp / 4) {
-                        case 1: conv_row_pairs<1>(z0, z1, rows, taps, first / 2, cqp, ckp, lane); break;
-                        case 2: conv_row_pairs<2>(z0, z1, rows, taps, first / 2, cqp, ckp, lane); break;
-                        case 3: conv_row_pairs<3>(z0, z1, rows, taps, first / 2, cqp, ckp, lane); break;
-                        case 4: conv_row_pairs<4>(z0, z1, rows, taps, first / 2, cqp, ckp, lane); break;
-                        default: conv_row_pairs<0>(z0, z1, rows, taps, first / 2, cqp, ckp, lane); break;
-                    }
-                    float z[2] = {z0.x + z0.y, z1.x + z1.y}, p[2];
+                for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        z[e] += __shfl_xor_sync(0xffffffffu, z[e], 8);
-                        z[e] += __shfl_xor_sync(0xffffffffu, z[e], 16);
-                        if (un * KEYS + 2 * (lane & 7) + e >= len) z[e] = -INFINITY;
-                    }
-                    const float top = fmaxf(m[y], warp_max(fmaxf(z[0], z[1])));
-                    // while every logit so far is -inf nothing has been summed: a finite stand-in keeps -inf - -inf away
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    fade[y] = fast_exp2(m[y] - ref);
-                    moved |= top != m[y];
-                    m[y] = top;
-                    p[0] = fast_exp2(z[0] - ref);
-                    p[1] = fast_exp2(z[1] - ref);
-                    l[y] = fmaf(l[y], fade[y], p[0] + p[1]);
-                    if constexpr (HALF) {
-                        constexpr float by = std::is_same_v<T, __half> ? FP16_WEIGHT : 1.0f;
-                        float a0[P::PIECES], a1[P::PIECES];
-                        split_pieces<T>(p[0] * by, a0);
-                        split_pieces<T>(p[1] * by, a1);
-                        // the four lanes that hold these keys write a piece each
-                        float w0 = a0[0], w1 = a1[0];
+                    for (int s = 8; s < 8 * SHARES; s <<= 1) z[e] += __shfl_xor_sync(0xffffffffu, z[e], s);
+                    if (un * KEYS + 2 * pair + e >= len) z[e] = -INFINITY;
+                }
+                float top = fmaxf(z[0], z[1]);
 #pragma unroll
-                        for (int i = 1; i < P::PIECES; ++i)
-                            if (lane >> 3 == i) { w0 = a0[i]; w1 = a1[i]; }
-                        if (lane >> 3 < P::PIECES)
-                            *reinterpret_cast<uint32_t*>(p_sm + (y * P::STRIDE + (lane >> 3)) * P_PITCH + 2 * (lane & 7)) = pack2<T>(w0, w1);
-                    } else {
-                        if (lane < 8) *reinterpret_cast<float2*>(p_sm + y * KEYS + 2 * lane) = make_float2(p[0], p[1]);
-                    }
+                for (int s = 1; s < 8; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                top = fmaxf(m, top);
+                // while every logit so far is -inf nothing has been summed: a finite stand-in keeps -inf - -inf away
+                const float ref = top == -INFINITY ? 0.0f : top, fade = fast_exp2(m - ref);
+                const bool moved = __any_sync(0xffffffffu, top != m);
+                m = top;
+                p[0] = fast_exp2(z[0] - ref);
+                p[1] = fast_exp2(z[1] - ref);
+                l = fmaf(l, fade, p[0] + p[1]);
+                if constexpr (HALF) {
+                    constexpr float by = std::is_same_v<T, __half> ? FP16_WEIGHT : 1.0f;
+                    float a0[P::PIECES], a1[P::PIECES];
+                    split_pieces<T>(p[0] * by, a0);
+                    split_pieces<T>(p[1] * by, a1);
+                    // the lanes that hold these keys share the pieces out
+#pragma unroll
+                    for (int i = 0; i < P::PIECES; ++i)
+                        if (i % SHARES == share) *reinterpret_cast<uint32_t*>(p_sm + (my_head * P::STRIDE + i) * P_PITCH + 2 * pair) = pack2<T>(a0[i], a1[i]);
+                } else {
+                    if (share == 0) *reinterpret_cast<float2*>(p_sm + my_head * KEYS + 2 * pair) = make_float2(p[0], p[1]);
                 }
                 __syncwarp();
                 if constexpr (HALF) {
                     if (moved) {
-                        float f0 = fade[0], f1 = fade[0];
-#pragma unroll
-                        for (int y = 1; y < GT; ++y) {
-                            if (2 * t4 / P::STRIDE == y) f0 = fade[y];
-                            if ((2 * t4 + 1) / P::STRIDE == y) f1 = fade[y];
-                        }
+                        // the head of this lane's two columns
+                        const int y = 2 * t4 / P::STRIDE;
+                        const float f = __shfl_sync(0xffffffffu, fade, (y < GT ? y : 0) * 8 * SHARES);
 #pragma unroll
                         for (int i = 0; i < V::CHUNKS; ++i)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) { o[i][j][0] *= f0; o[i][j][1] *= f1; o[i][j][2] *= f0; o[i][j][3] *= f1; }
+                            for (int j = 0; j < 4; ++j) { o[i][j][0] *= f; o[i][j][1] *= f; o[i][j][2] *= f; o[i][j][3] *= f; }
                     }
                     const uint32_t* col_p = reinterpret_cast<const uint32_t*>(p_sm + g * P_PITCH) + t4;
                     values.multiply(o, col_p[0], col_p[4]);
                 } else {
 #pragma unroll
-                    for (int y = 0; y < GT; ++y)
+                    for (int y = 0; y < GT; ++y) {
+                        const float f = __shfl_sync(0xffffffffu, fade, y * 8 * SHARES);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[y][0][e] *= fade[y];
+                        for (int e = 0; e < 4; ++e) o[y][0][e] *= f;
+                    }
 #pragma unroll
                     for (int i = 0; i < V::STEPS; ++i) {
                         float f[4];
@@ -292,12 +284,18 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
         }
         const bool all = u0 == 0 && u1 == tiles;                     // the whole line: nothing to join
         const long part = me + (long)b * lines + line;
+#pragma unroll
+        for (int s = 1; s < 8; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+        float sums[GT];
+#pragma unroll
+        for (int y = 0; y < GT; ++y) sums[y] = __shfl_sync(0xffffffffu, l, y * 8 * SHARES);
+        if (lane % (8 * SHARES) == 0 && !all) a.part_ml[part * GT + my_head] = make_float2(m, l);
         // Stores EPL elements of head y from element e0 on.
         auto store = [&](int y, int e0, const float* f) {
             if (all) {
                 float r[EPL];
 #pragma unroll
-                for (int e = 0; e < EPL; ++e) r[e] = f[e] / l[y];
+                for (int e = 0; e < EPL; ++e) r[e] = f[e] / sums[y];
                 *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((long)b * c.H + h0 + y) * c.D + e0) = pack16<T>(r);
             } else {
                 float* to = a.part_o + (part * GT + y) * c.D + e0;
@@ -305,12 +303,6 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
                 for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
             }
         };
-#pragma unroll
-        for (int y = 0; y < GT; ++y) {
-#pragma unroll
-            for (int s = 1; s < 8; s <<= 1) l[y] += __shfl_xor_sync(0xffffffffu, l[y], s);
-            if (lane == 0 && !all) a.part_ml[part * GT + y] = make_float2(m[y], l[y]);
-        }
         if constexpr (HALF) {
             constexpr float by = std::is_same_v<T, __half> ? 1.0f / FP16_WEIGHT : 1.0f;
 #pragma unroll
