@@ -50,11 +50,12 @@ class TritonConvAttention(nn.Module):
         prompt = Q.size(2) != 1
         if prompt and not batch.from_empty:
             raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
+        longest = cache.longest(batch, max_length)
         cache.append(batch, K, V, Q, layer)
         if prompt:
             group = Q.size(1) // K.size(1)
             if group > 1:
                 K, V = K.repeat_interleave(group, dim=1), V.repeat_interleave(group, dim=1)
             return ops.conv_attn_fwd(Q, K, V, self.weight, True, softmax_scale), None
-        return ops.conv_attn_decode_fwd(*cache.layer(layer), self.weight, softmax_scale, batch.max_length if max_length is None else max_length,
+        return ops.conv_attn_decode_fwd(*cache.layer(layer), self.weight, softmax_scale, longest,
                                         slots=batch.slot_ids), None

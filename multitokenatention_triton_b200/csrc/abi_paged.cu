@@ -17,6 +17,7 @@ int describe(PagedCache* c, const char* K, const void* q_hist, const void* k, co
     MTA_REQUIRE(D >= 8 && D % 8 == 0 && D <= most, "%s: head dimension %d; a multiple of 8 up to %d is wanted", K, D, most);
     MTA_REQUIRE(max_length >= 0 && max_length <= (long)table_width * page, "%s: a longest sequence of %d tokens, but a table row holds %ld", K, max_length,
                 (long)table_width * page);
+    MTA_REQUIRE((long)table_width * page <= 1L << 30, "%s: table rows of %d pages of %d tokens; sequences of up to 2^30 tokens are supported", K, table_width, page);
     MTA_REQUIRE(q_hist && k && v && table && lengths, "%s: null pointer", K);
     MTA_REQUIRE(aligned16(q_hist) && aligned16(k) && aligned16(v), "%s: queries, keys and values must begin on 16-byte boundaries", K);
     c->q_hist = q_hist; c->k = k; c->v = v; c->table = table; c->lengths = lengths; c->slot_ids = slot_ids;
@@ -35,8 +36,9 @@ int check_taps(const char* K, int cq, int ck, int rows, int ring) {
     return MTA_OK;
 }
 
-int check_batch(const char* K, int B) {
+int check_batch(const char* K, int B, int max_length) {
     MTA_REQUIRE(B <= DECODE_MAX_BATCH, "%s: %d batch rows; at most %d are supported in one call", K, B, DECODE_MAX_BATCH);
+    MTA_REQUIRE((long)B * max_length <= 1L << 34, "%s: %d rows of up to %d tokens; at most 2^34 tokens together are supported", K, B, max_length);
     return MTA_OK;
 }
 }  // namespace
@@ -113,7 +115,7 @@ int mta_conv_attn_decode_fwd(const void* q_hist, const void* k_pages, const void
         return rc;
     MTA_REQUIRE(dtype_ok(w_dtype), "%s: unknown dtype code %d of the weight", K, w_dtype);
     if (int rc = check_taps(K, cq, ck, cq, ring)) return rc;
-    if (int rc = check_batch(K, B)) return rc;
+    if (int rc = check_batch(K, B, max_length)) return rc;
     if (B == 0) return MTA_OK;
     MTA_REQUIRE(w && o && aligned16(o), "%s: null or unaligned pointer", K);
     const size_t need = conv_attn_decode_workspace(B, H, kv_heads, D, cq, max_length);
@@ -142,7 +144,7 @@ int mta_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages,
     MTA_REQUIRE(cq2 >= 1 && cq2 <= DECODE_MAX_ROWS && cq <= DECODE_MAX_ROWS, "%s: %d and %d query taps", K, cq, cq2);
     if (int rc = check_taps(K, cq, ck, cq + cq2 - 1, ring)) return rc;
     if (int rc = check_taps(K, cq2, ck2, cq + cq2 - 1, ring)) return rc;
-    if (int rc = check_batch(K, B)) return rc;
+    if (int rc = check_batch(K, B, max_length)) return rc;
     if (B == 0) return MTA_OK;
     MTA_REQUIRE(w1 && W1 && w2 && W2 && o, "%s: null pointer", K);
     size_t need = 0;

@@ -186,6 +186,7 @@ class MTAAttentionTriton(nn.Module):
         prompt = xq.size(2) != 1
         if prompt and not batch.from_empty:
             raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
+        longest = cache.longest(batch, max_length)
         cache.append(batch, xk, xv, xq, layer)
         if prompt:
             group = xq.size(1) // xk.size(1)
@@ -194,7 +195,7 @@ class MTAAttentionTriton(nn.Module):
             return self.forward(xq, xk, xv, None, None)
         out = ops.mta_decode_fwd(*cache.layer(layer), self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
                                  self.mta_conv_after_sm_triton.effective_weight(), self.wposm_triton.weight,
-                                 batch.max_length if max_length is None else max_length, slots=batch.slot_ids)
+                                 longest, slots=batch.slot_ids)
         return out.transpose(1, 2)
 
     def reset_mta_parameters(self, init_std=None):

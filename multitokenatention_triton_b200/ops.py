@@ -514,6 +514,7 @@ def mta_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
         raise MTALibraryError(f"mta_decode: expected conv weights ({H},cq,ck) and head mixes ({H},{H}), got {tuple(s1)}, {tuple(W1.shape)}, {tuple(s2)}, "
                               f"{tuple(W2.shape)}")
     taps = (s1[1], s1[2], s2[1], s2[2])
+    max_length = int(max_length)
     # zero bytes: a shape that the call refuses, with the reason
     nbytes = _size("mta_decode_workspace_bytes", B, H, kv_heads, D, *taps, max_length)
     out, workspace, nbytes = _decode_buffers("mta_decode", q_hist, B, H, D, dev, out, workspace, nbytes)
@@ -537,6 +538,7 @@ def conv_attn_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: t
         raise MTALibraryError(f"conv_attn_decode: expected a weight ({H},cq,ck), got {tuple(shape)}")
     if softmax_scale is None:
         softmax_scale = 1.0 / (D ** 0.5)
+    max_length = int(max_length)
     nbytes = _size("mta_conv_attn_decode_workspace_bytes", B, H, kv_heads, D, shape[1], shape[2], max_length)
     out, workspace, nbytes = _decode_buffers("conv_attn_decode", q_hist, B, H, D, dev, out, workspace, nbytes)
     _launch(dev, "mta_conv_attn_decode_fwd", lib().mta_conv_attn_decode_fwd, q_hist.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(),

@@ -259,6 +259,14 @@ class PagedKVCache:
             if self._stamp[s] != stamp:
                 raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend()")
 
+    def longest(self, batch: CacheBatch, max_length: Optional[int]) -> int:
+        """The longest length that an attention call over the batch is to serve: the batch's own, or a larger one."""
+        if max_length is None:
+            return batch.max_length
+        if not batch.max_length <= max_length <= self.max_length:
+            raise MTALibraryError(f"max_length = {max_length}, but the batch has {batch.max_length} tokens and the cache at most {self.max_length}")
+        return max_length
+
     def append(self, batch: CacheBatch, xk: torch.Tensor, xv: torch.Tensor, xq: torch.Tensor, layer: int = 0) -> None:
         """Writes the batch's new tokens of one layer: xk, xv (B,kv heads,T,D), xq (B,H,T,D) with T >= every count; tokens behind a row's count are
         not read."""

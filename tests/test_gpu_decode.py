@@ -153,6 +153,45 @@ def test_on_another_stream():
     check(pool, b, range(2), w, 0.125, False)
 
 
+def test_calls_at_once_on_two_streams():
+    pools = [Pool([700, 90], 8, 8, 64, 64, 8, torch.bfloat16, DEV, seed=i) for i in range(2)]
+    w = mta_weights(8, (6, 11), (3, 3), torch.bfloat16, DEV)
+    alone = [ops.mta_decode_fwd(*p.tensors(), *w, 700) for p in pools] + [ops.conv_attn_decode_fwd(*p.tensors(), w[0], 0.125, 700) for p in pools]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = {}
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i] = ops.mta_decode_fwd(*pools[i].tensors(), *w, 700)
+                outs[2 + i] = ops.conv_attn_decode_fwd(*pools[i].tensors(), w[0], 0.125, 700)
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert torch.equal(outs[i], alone[i])
+
+
+def test_an_append_is_seen_by_the_attention_behind_it():
+    """The calls of a step follow one another without a pause: what the append writes is read, over many steps."""
+    pool = Pool([64, 17], 8, 8, 64, 64, 8, torch.bfloat16, DEV, spare=4)
+    free = [p for p in range(pool.k_pages.shape[0]) if p not in {int(x) for s, n in enumerate(pool.lens) for x in pool.table[s, :-(-n // 64)]}]
+    pool.table[0, 1] = free[0]
+    w = mta_weights(8, (6, 11), (3, 3), torch.bfloat16, DEV)
+    new = torch.randn(40, 3, 2, 8, 1, 64, device=DEV).bfloat16()
+    outs = []
+    for q, k, v in new:
+        pool.lengths += 1
+        ops.cache_append(k, v, q, *(pool.tensors()[i] for i in (1, 2, 0, 3, 4)))
+        outs.append((ops.mta_decode_fwd(*pool.tensors(), *w, 110), ops.conv_attn_decode_fwd(*pool.tensors(), w[0], 0.125, 110)))
+    for s in range(2):
+        q, k, v = (torch.cat([old[s], new[:, i, s, :, 0].transpose(0, 1)], 1) for i, old in enumerate((pool.q, pool.k, pool.v)))
+        for n in (1, 2, 25, 39, 40):
+            have = pool.lens[s] + n
+            for kind in (0, 1):
+                ref, bound = token64(q[:, :have], k[:, :have], v[:, :have], w[0], 0.125, *(() if kind else w[1:]))
+                assert_near(outs[n - 1][kind][s, :, 0], ref, bound, f"slot {s}, {n} tokens on")
+    _lib.cache_status()
+
+
 def test_captured_graphs_follow_lengths_and_tables():
     """Two graphs captured with workspaces of their own serve shorter and longer sequences than those they were captured with."""
     pool = Pool([100, 30], 8, 8, 64, 32, 8, torch.bfloat16, DEV)

@@ -179,6 +179,16 @@ def test_random_life_of_a_cache(plain_copies, seed):
         assert counts == c._refs and sorted(c._free_pages) == [p for p in range(20) if counts[p] == 0]
 
 
+def test_longest_length_of_a_call():
+    c = small()
+    a = c.add()
+    batch = c.extend([a], 20)
+    assert c.longest(batch, None) == 20 and c.longest(batch, 20) == 20 and c.longest(batch, 96) == 96
+    for bad in (19, 97, -1):
+        with pytest.raises(MTALibraryError, match="max_length"):
+            c.longest(batch, bad)
+
+
 def test_empty_problems_and_bad_arguments_of_the_c_calls():
     L = _lib.lib()
     z, one = ctypes.c_void_p(0), ctypes.c_void_p(16)
@@ -190,7 +200,7 @@ def test_empty_problems_and_bad_arguments_of_the_c_calls():
     assert append(B=0) == 0 and append(T=0) == 0
     for bad in (dict(T=-1), dict(B=-1), dict(B=3), dict(slots=0), dict(width=0), dict(pages=0), dict(page=24), dict(page=8), dict(ring=0), dict(H=0), dict(kv=0),
                 dict(kv=3), dict(D=0), dict(D=20), dict(D=264), dict(D=136, dtype=0), dict(dtype=3), dict(k=z), dict(k=ctypes.c_void_p(24)),
-                dict(strides=(ctypes.c_longlong * 9)(*[60] * 9)), dict(width=1 << 20, page=65536)):
+                dict(strides=(ctypes.c_longlong * 9)(*[60] * 9)), dict(width=1 << 20, page=65536), dict(width=1 << 15, page=65536)):
         assert append(**bad) == 1, bad
         assert L.mta_last_error()
 
