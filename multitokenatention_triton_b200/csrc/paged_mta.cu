@@ -992,7 +992,7 @@ int make_plan(Plan* p, int B, int H, int kv_heads, int D, int cq, int ck, int cq
         auto rounds = [&](int copies) { return (float)((H / p->gt * copies + ROLE_WARPS - 1) / ROLE_WARPS) / copies; };
         for (int copies = 2; copies <= tile / KEYS; copies *= 2)
             if (rounds(copies) < rounds(p->copies)) p->copies = copies;
-        for (p->kv_together = kv_heads; p->kv_together >= 1 && !fits; p->kv_together = p->kv_together / 2) {
+        for (p->kv_together = kv_heads; p->kv_together >= 1 && !fits; --p->kv_together) {
             p->score_bytes = score_smem(B, H, group, kv_heads, p->kv_together, tile, cq, ck, cq2).bytes;
             p->value_bytes = value_smem(B, H, D, tile, cq2, ck2, p->copies).bytes;
             // a smaller tile before the heads are taken in parts (of whole pairs)
