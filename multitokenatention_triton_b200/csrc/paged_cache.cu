@@ -1,4 +1,6 @@
-// Writes into a paged cache: new tokens' keys, values and queries, and copies of whole pages.  Both only move bytes.
+// Writes into a paged cache: new tokens' keys, values and queries, and copies of whole pages.  Both only move bytes, and HBM bounds
+// them: prompts of 8 x up to 4096 tokens, 16 heads of 128 in bf16 64 us = 5.9 TB/s read and written, 1500 pages of 64 tokens 241 us = 6.5 TB/s;
+// one token of 64 sequences 2.2 us, eight pages 2.4 us, their launches.
 #include "paged.cuh"
 
 namespace mta {

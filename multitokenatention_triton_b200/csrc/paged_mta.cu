@@ -6,14 +6,19 @@
 //   y[h,k]   = sum_{i,j} w2[h,i,j] p[h,i,k+j-(ck2-1)/2],  k <= t
 //   out[o]   = sum_k (sum_h W2[o,h] y[h,k]) v[o,k]
 //
-// The rows before the newest are computed again from the last R queries instead of being kept: with the queries as the eight
-// columns of an mma they cost no byte more, and a cache that holds keys, values and R queries can be forked or moved at any token.
+// The rows before the newest are computed again from the last R queries instead of being kept: an mma has sixteen query rows
+// anyway, so they cost no byte more, and a cache that holds keys, values and R queries can be forked or moved at any token.
 // Both head mixes need all heads of a key, the softmax all keys of a row, so the work is three kernels:
 //   scores  block = a run of key tiles, all heads: scores, conv, head mix; logits to the workspace (float32, base 2),
 //           maximum and sum of every (row, head) of the run
 //   values  the same runs: joins the maxima and sums of all runs, probabilities, conv, head mix, product with the values
 //   join    adds the runs' outputs
 // Keys and values are read once; the logits add 4 cq2 bytes written and read, mostly in L2, to the 4 D of keys and values in 16 bits.
+//
+// Measured, bf16, D 128, taps 6x11 and 3x3 (a graph of calls): 16 sequences of 8192 tokens, 32 heads 462 us, 4.65 TB/s of keys and values
+// (scores 267, values 212, join 8 under the profiler); 8 sequences of 1024 to 4096 tokens, 16 heads 80 us; one of 301 tokens 27 us.
+// The long batch is bound by instructions and their latency (scores, when they took 291 us: 276 with every load from L1, 213 with no convs
+// and mixes), the short ones by the chain of stages: a run of 155 keys has three.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -22,8 +27,9 @@ namespace mta {
 namespace {
 
 // A block is one per SM, half of its warps on memory and half on arithmetic: eight stream keys (values) and multiply, eight run the
-// convs, head mixes and softmaxes of the tile before (after).  With all sixteen doing one after the other memory stood still for a third of
-// the time: 770 us for 16 sequences of 8192 tokens and 32 heads.
+// convs, head mixes and softmaxes of the tile before (after).  Two blocks of eight warps that did one after the other left the
+// memory idle in every block's second half: 770 us for the long batch.  Asking L2 for the next tile ahead made it slower (1.47 GB
+// read from memory instead of 1.11).
 constexpr int ROLE_WARPS = 8, ROLE_THREADS = ROLE_WARPS * 32, THREADS = 2 * ROLE_THREADS;
 // Named barriers: a stage's buffer is full or empty (by the stage's parity), and those of one half alone.
 enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_MATH = 5, BAR_MEMORY = 6 };
@@ -46,9 +52,10 @@ __host__ __device__ inline int halo(int x) { return (x + KEYS - 1) / KEYS * KEYS
 
 // The scores of two tiles and their neighbours: a ring of `keys` positions, so that one tile's scores are written while the conv reads
 // the other's, and what tiles share is computed once; keys lie at their number plus a multiple of 16 that lets a sequence begin
-// where the one before ended.  Where not all heads fit, the tiles (of one group of heads after another) have a ring each.  Two heads stand side by side, which lets one packed FMA serve both.  Keys (4i, 4i + 1) lie in the first half of a
-// row, (4i + 2, 4i + 3) in the second, 16 bytes each: the conv's threads, four keys apart, read neighbouring 16 bytes.  The pads
-// put the rows and halves that an accumulator writes at once into different banks.
+// where the one before ended.  Where not all heads fit, the tiles (of one group of heads after another) have a ring each.  Two heads
+// stand side by side, which lets one packed FMA serve both.  Keys (4i, 4i + 1) lie in the first half of a row, (4i + 2, 4i + 3) in
+// the second, 16 bytes each: the conv's threads, four keys apart, read neighbouring 16 bytes.  The pads put the rows and halves
+// that an accumulator writes at once into different banks.
 // Windows begin on multiples of four keys: taps have up to three zeros in front (`lead`) for that, and zeros behind up to `taps`.
 __host__ __device__ inline int lead(int ck) { return (4 - (ck - 1) / 2 % 4) % 4; }
 __host__ __device__ inline int score_taps(int ck) { return round4(ck + lead(ck)); }
@@ -770,7 +777,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
 #pragma unroll
                     for (int i = 0; i < V::STEPS; ++i) {
                         float f[4];
-                        unpack16<float>(values[n_].r[i], f);
+                        unpack16(values[n_].r[i], f);
 #pragma unroll
                         for (int y = 0; y < GT; ++y) {
                             const float p = weights[((h0 + y) << a.shift) + (unit + n_) * KEYS + i * V::SUBS + lane / V::ROWLANES];
