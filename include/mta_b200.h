@@ -270,7 +270,8 @@ int mta_host_pipeline_release(void);
  * queries are read (at most 32); kernels have at most 33 key taps, odd or even, centred as mta_conv2d_fwd centres them; H <= 128.
  * mta_conv_attn_decode_fwd is the conv attention (mta_conv_attn_fwd, causal) likewise; it reads the last cq queries.
  * Both: an empty sequence gets zeros; no length exceeds max_length (which sizes the workspace and the split of the work: inside a
- * captured graph pass the longest that the graph is to serve); at most 1024 rows.  Sums, softmax statistics, scores and weights are float32;
+ * captured graph pass the longest that the graph is to serve; up to 2^30, times the rows up to 2^34); at most 1024 rows.  A workspace serves one
+ * call at a time.  Sums, softmax statistics, scores and weights are float32;
  * the result is rounded once, so it is nearer to exact than the whole-sequence forward, which rounds between stages.
  */
 int mta_cache_append(const void* k, const void* v, const void* q, const long long* strides, const int* counts, void* k_pages, void* v_pages,

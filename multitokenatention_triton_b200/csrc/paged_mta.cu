@@ -59,12 +59,15 @@ __host__ __device__ inline int halo(int x) { return (x + KEYS - 1) / KEYS * KEYS
 // Windows begin on multiples of four keys: taps have up to three zeros in front (`lead`) for that, and zeros behind up to `taps`.
 __host__ __device__ inline int lead(int ck) { return (4 - (ck - 1) / 2 % 4) % 4; }
 __host__ __device__ inline int score_taps(int ck) { return round4(ck + lead(ck)); }
+// Keys behind a tile that its windows touch, those that meet zeros included: they have to be scores of the same sequence, since a zero times
+// what another sequence left there is no zero where that is not finite.
+__host__ __device__ inline int halo_right(int ck) { return halo(score_taps(ck) - (ck - 1) / 2 - lead(ck)); }
 // From one pair of heads' taps to the next pair's: 16 bytes more than they take, so that pairs lie in different banks.
 __host__ __device__ inline int pair_taps(int cq, int ck) { return cq * score_taps(ck) + 2; }
 struct ScoreRing {
     int keys, half, row;   // floats of half a row and of a row
     __host__ __device__ ScoreRing(int tile, int ck, bool whole) {
-        keys = (halo((ck - 1) / 2) + tile + halo(ck - 1 - (ck - 1) / 2)) * (whole ? 2 : 1);
+        keys = (halo((ck - 1) / 2) + tile + halo_right(ck)) * (whole ? 2 : 1);
         half = keys + (keys % 32 == 0 ? 8 : 24);
         row = 2 * half + 8;
     }
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     extern __shared__ __align__(16) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = score_taps(a.ck);
-    const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo(a.ck - 1 - left), first_tap = lead(a.ck);
+    const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo_right(a.ck), first_tap = lead(a.ck);
     const bool whole = a.kv_together == c.kv_heads;              // all heads at once: what tiles share stays in the ring
     const ScoreRing ring(tile, a.ck, whole);
     const ScoreSmem m = score_smem(a.B, H, group, c.kv_heads, a.kv_together, tile, a.cq, a.ck, a.cq2);
@@ -265,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     float2 *t_sm = reinterpret_cast<float2*>(smem + m.taps), *ml = reinterpret_cast<float2*>(smem + m.ml);
     int *before = reinterpret_cast<int*>(smem + m.before), *lens = before + a.B + 1;
 
-    // positions that hold no score yet are read with taps of zero, or for keys behind the run: they have to be finite
+    // places that hold no score yet are read for keys behind the run, whose results are dropped: zeros, so that nothing undefined is read
     for (int i = threadIdx.x; i < (int)((m.c - m.s) / 16); i += THREADS) reinterpret_cast<float4*>(s_sm)[i] = make_float4(0, 0, 0, 0);
     pdl_wait();
     count_tiles(c, a.B, 4, before, lens);

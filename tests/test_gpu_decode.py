@@ -117,6 +117,24 @@ def test_sharp_softmax_rows(spread):
     check(pool, ops.conv_attn_decode_fwd(*pool.tensors(), w[0], 0.125, 600), range(1), w, 0.125, False)
 
 
+@pytest.mark.parametrize("kernel,kernel2", [((1, 1), (1, 1)), ((6, 11), (3, 3)), ((2, 33), (2, 33)), ((3, 32), (2, 2))])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+def test_a_sequence_that_is_not_finite_leaves_the_others_alone(kernel, kernel2, poison):
+    """Every other sequence of a batch whose runs hold several has keys and values that are no numbers."""
+    lens = [20 + 7 * (i % 6) for i in range(90)]
+    pool = Pool(lens, 4, 4, 64, 16, 8, torch.bfloat16, DEV)
+    for s in range(0, 90, 2):
+        pages = pool.table[s, :-(-lens[s] // 16)].long()
+        pool.k_pages[pages], pool.v_pages[pages] = poison, poison
+    w = mta_weights(4, kernel, kernel2, torch.bfloat16, DEV)
+    for mta in (True, False):
+        got = ops.mta_decode_fwd(*pool.tensors(), *w, max(lens)) if mta else ops.conv_attn_decode_fwd(*pool.tensors(), w[0], 0.125, max(lens))
+        for s in range(1, 90, 2):
+            ref, bound = token64(pool.q[s], pool.k[s], pool.v[s], w[0], 0.125, *(w[1:] if mta else ()))
+            assert_near(got[s, :, 0], ref, bound, f"row {s} of {lens[s]} tokens")
+        assert not bool(torch.isfinite(got[::2]).any())
+
+
 def test_results_do_not_change_from_call_to_call():
     pool = Pool([900, 411, 64], 16, 16, 128, 64, 8, torch.bfloat16, DEV)
     w = mta_weights(16, (6, 11), (3, 3), torch.bfloat16, DEV)
