@@ -212,13 +212,18 @@ template <int DMAX> struct ValueTileF32 {
 // 32 bytes at 256 p + 32 g, as chunks 2p and 2p + 1 (DMAX 64: 16 bytes at 16 g), of keys 2t, 2t + 1, 2t + 8 and 2t + 9, and pairs neighbouring keys'
 // halves with one byte permute each; mma (c, j) has element e + j as its row g and e + j + 4 as its row g + 8, e = element(c, g).
 //
-// The B operand's eight columns hold the weights of GT heads, each split into PIECES 16-bit numbers that add up to it: columns
-// y * STRIDE + i, i < PIECES, so that an mma that has eight columns anyway multiplies weights of 24 (bf16) or 33 bits (fp16) with the
-// values at no cost; with four heads two pieces fit, 16 bits or 22, whose rounding of 2^-16 at most is far below the 2^-8 of
-// a bf16 result.  Against FMAs on unpacked values (8 conversions and 4 packed FMAs for 8 elements and head) this takes a half of the
-// instructions for one head, a sixth for four.
+// The B operand's eight columns hold the weights of GT heads, each split into three 16-bit numbers that add up to it: columns
+// y * STRIDE + i, so that an mma that has eight columns anyway multiplies weights of 24 (bf16) or 33 bits (fp16) with the
+// values at no cost.  Four heads have two columns each: a second mma (set) adds their third pieces.  Its first column of a head is no
+// zero but the other half of the first piece, which makes that column the product with the first piece alone; see split_pieces.
+// Two pieces (16 bits in bf16) were enough for a result of 8 bits unless it is a small difference of large terms.
+// Against FMAs on unpacked values (8 conversions and 4 packed FMAs for 8 elements and head) this takes a half of the
+// instructions for one head, a fifth for four.
 template <int GT> struct Pieces {
-    static constexpr int PIECES = GT == 4 ? 2 : 3, STRIDE = 8 / (GT == 1 ? 2 : GT);
+    static constexpr int PIECES = 3, SETS = GT == 4 ? 2 : 1, STRIDE = 8 / (GT == 1 ? 2 : GT);
+    // Piece in column STRIDE * y + i of a set, i < WIDTH.
+    static constexpr int WIDTH = SETS == 2 ? 2 : PIECES;
+    static __device__ __forceinline__ int piece_of(int set, int i) { return set == 1 && i == 1 ? 2 : i; }
 };
 template <typename T, int DMAX> struct ValueTile {
     static constexpr int CHUNKS = DMAX / 64;
@@ -256,7 +261,7 @@ template <typename T, int DMAX> struct ValueTile {
         }
     }
     // acc[c][j] += values x weights: [0], [1] element(c, g) + j, columns 2t and 2t + 1; [2], [3] element(c, g) + j + 4.
-    __device__ __forceinline__ void multiply(float (&acc)[CHUNKS][4][4], uint32_t b0, uint32_t b1) const {
+    template <int SETS> __device__ __forceinline__ void multiply(float (&acc)[CHUNKS][4][4], const uint32_t (&b)[SETS][2]) const {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
 #pragma unroll
@@ -264,19 +269,19 @@ template <typename T, int DMAX> struct ValueTile {
                 const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
                 const uint32_t lo[4] = {j < 2 ? r[0][c].x : r[0][c].y, j < 2 ? r[1][c].x : r[1][c].y, j < 2 ? r[2][c].x : r[2][c].y, j < 2 ? r[3][c].x : r[3][c].y};
                 const uint32_t hi[4] = {j < 2 ? r[0][c].z : r[0][c].w, j < 2 ? r[1][c].z : r[1][c].w, j < 2 ? r[2][c].z : r[2][c].w, j < 2 ? r[3][c].z : r[3][c].w};
-                mma_16816<T>(acc[c][j], __byte_perm(lo[0], lo[1], sel), __byte_perm(hi[0], hi[1], sel), __byte_perm(lo[2], lo[3], sel),
-                             __byte_perm(hi[2], hi[3], sel), b0, b1);
+                const uint32_t a[4] = {__byte_perm(lo[0], lo[1], sel), __byte_perm(hi[0], hi[1], sel), __byte_perm(lo[2], lo[3], sel), __byte_perm(hi[2], hi[3], sel)};
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) mma_16816<T>(acc[c][j], a[0], a[1], a[2], a[3], b[s][0], b[s][1]);
             }
         }
     }
 };
-// x as a sum of PIECES numbers of type T, the i-th of them.
-template <typename T, int PIECES> __device__ __forceinline__ void split_pieces(float x, float (&piece)[PIECES]) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        piece[i] = round_to<T>(x);
-        x -= piece[i];
-    }
+// x as a sum of three numbers of type T; with two sets the first, which both have, counts twice.
+template <typename T, int SETS> __device__ __forceinline__ void split_pieces(float x, float (&piece)[3]) {
+    piece[0] = round_to<T>(SETS == 2 ? 0.5f * x : x);
+    x = fmaf(-(float)SETS, piece[0], x);
+    piece[1] = round_to<T>(x);
+    piece[2] = round_to<T>(x - piece[1]);
 }
 
 // 2^x to a relative 2^-22; 0 below the smallest normal number.

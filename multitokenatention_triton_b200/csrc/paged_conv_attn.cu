@@ -59,7 +59,7 @@ template <typename T, int DMAX, int NT> constexpr int query_bytes = sizeof(T) ==
 // GT query heads that share a kv head, each with cq rows rounded up to pairs; NT * 8 >= all their rows of scores.
 template <typename T, int DMAX, int GT, int NT> __host__ __device__ constexpr size_t conv_attn_warp_smem(int cq, int ck) {
     return (size_t)query_bytes<T, DMAX, NT> + (size_t)NT * 4 * RING_PITCH * 4 + (size_t)GT * ((cq + 1) / 2) * taps_pitch(ck) * 8 +
-           (sizeof(T) == 2 ? 8 * P_PITCH * 2 : GT * KEYS * 4);
+           (sizeof(T) == 2 ? Pieces<GT>::SETS * 8 * P_PITCH * 2 : GT * KEYS * 4);
 }
 
 // Two neighbouring keys of the conv, summed over the pairs of tap rows i, i + every, ...: .x the first rows of the pairs, .y the second.
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
     char* q_sm = mine;
     float* s_sm = reinterpret_cast<float*>(mine + query_bytes<T, DMAX, NT>);
     float2* w_sm = reinterpret_cast<float2*>(s_sm + NT * 4 * RING_PITCH);       // [head][pair of tap rows][key tap]
-    T* p_sm = reinterpret_cast<T*>(w_sm + GT * cqp * taps_pitch(a.ck));                      // [column][key]; float32: [head][key]
+    T* p_sm = reinterpret_cast<T*>(w_sm + GT * cqp * taps_pitch(a.ck));                      // [set][column][key]; float32: [head][key]
     int* before = reinterpret_cast<int*>(smem + WARPS * conv_attn_warp_smem<T, DMAX, GT, NT>(a.cq, a.ck));
     int* lens = before + a.B + 1;
 
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
                                   j < a.ck && 2 * pair + 1 < a.cq ? load_weight(a.w, at + a.ck, a.w_dtype) * a.scale : 0.0f);
         }
         if constexpr (HALF) {
-            for (int i = lane; i < 8 * P_PITCH / 2; i += 32) reinterpret_cast<uint32_t*>(p_sm)[i] = 0;      // columns that no piece fills
+            for (int i = lane; i < P::SETS * 8 * P_PITCH / 2; i += 32) reinterpret_cast<uint32_t*>(p_sm)[i] = 0;      // columns that no piece fills
         }
         __syncwarp();
 
@@ -243,12 +243,15 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
                 if constexpr (HALF) {
                     constexpr float by = std::is_same_v<T, __half> ? FP16_WEIGHT : 1.0f;
                     float a0[P::PIECES], a1[P::PIECES];
-                    split_pieces<T>(p[0] * by, a0);
-                    split_pieces<T>(p[1] * by, a1);
+                    split_pieces<T, P::SETS>(p[0] * by, a0);
+                    split_pieces<T, P::SETS>(p[1] * by, a1);
                     // the lanes that hold these keys share the pieces out
 #pragma unroll
-                    for (int i = 0; i < P::PIECES; ++i)
-                        if (i % SHARES == share) *reinterpret_cast<uint32_t*>(p_sm + (my_head * P::STRIDE + i) * P_PITCH + 2 * pair) = pack2<T>(a0[i], a1[i]);
+                    for (int s = 0; s < P::SETS; ++s)
+#pragma unroll
+                        for (int i = 0; i < P::WIDTH; ++i)
+                            if (i % SHARES == share)
+                                *reinterpret_cast<uint32_t*>(p_sm + (s * 8 + my_head * P::STRIDE + i) * P_PITCH + 2 * pair) = pack2<T>(a0[P::piece_of(s, i)], a1[P::piece_of(s, i)]);
                 } else {
                     if (share == 0) *reinterpret_cast<float2*>(p_sm + my_head * KEYS + 2 * pair) = make_float2(p[0], p[1]);
                 }
@@ -263,8 +266,14 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
 #pragma unroll
                             for (int j = 0; j < 4; ++j) { o[i][j][0] *= f; o[i][j][1] *= f; o[i][j][2] *= f; o[i][j][3] *= f; }
                     }
-                    const uint32_t* col_p = reinterpret_cast<const uint32_t*>(p_sm + g * P_PITCH) + t4;
-                    values.multiply(o, col_p[0], col_p[4]);
+                    uint32_t w[P::SETS][2];
+#pragma unroll
+                    for (int s = 0; s < P::SETS; ++s) {
+                        const uint32_t* col_p = reinterpret_cast<const uint32_t*>(p_sm + (s * 8 + g) * P_PITCH) + t4;
+                        w[s][0] = col_p[0];
+                        w[s][1] = col_p[4];
+                    }
+                    values.multiply(o, w);
                 } else {
 #pragma unroll
                     for (int y = 0; y < GT; ++y) {

@@ -103,7 +103,7 @@ __host__ __device__ inline ValueSmem value_smem(int B, int H, int D, int tile, i
     size_t at = 0;
     m.p = at; at += (size_t)cq2 * H * prob_pitch(tile, ck2) * 4;
     m.y = at; at += (size_t)H * tile * 4;
-    m.a_one = (size_t)H * (3 * piece_pitch(tile) * 2);           // up to three pieces; float32: 4 bytes a key
+    m.a_one = (size_t)H * (3 * piece_pitch(tile) * 2);           // three pieces; float32: 4 bytes a key
     m.a = at; at += 2 * m.a_one;
     m.W = at; at += (size_t)H * round4(H) * 4;
     m.taps = at; at += (size_t)H * cq2 * round4(ck2) * 4;
@@ -728,13 +728,24 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                     for (int j = 0; j < 4; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.0f;
             }
             if constexpr (HALF) {
-                const int y = g / P::STRIDE, piece = g % P::STRIDE;
-                const bool on = y < GT && piece < P::PIECES;
-                const uint32_t* col = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + piece) * ap : 0)) + t4 + unit * 8;
+                const int y = g / P::STRIDE, column = g % P::STRIDE;
+                const bool on = y < GT && column < P::WIDTH;
+                const uint32_t* col[P::SETS];
+#pragma unroll
+                for (int s = 0; s < P::SETS; ++s)
+                    col[s] = reinterpret_cast<const uint32_t*>(weights + (on ? ((h0 + y) * P::PIECES + P::piece_of(s, column)) * ap : 0)) + t4 + unit * 8;
                 more = advance();
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    if (i == 0 || i < units) values[i].multiply(acc, on ? col[i * 8] : 0u, on ? col[i * 8 + 4] : 0u);
+                    if (i == 0 || i < units) {
+                        uint32_t w[P::SETS][2];
+#pragma unroll
+                        for (int s = 0; s < P::SETS; ++s) {
+                            w[s][0] = on ? col[s][i * 8] : 0u;
+                            w[s][1] = on ? col[s][i * 8 + 4] : 0u;
+                        }
+                        values[i].multiply(acc, w);
+                    }
                     if (more) load(i);
                 }
                 if (final) {
@@ -922,7 +933,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                     if constexpr (HALF) {
                         float f[4][P::PIECES];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) split_pieces<T>(std::is_same_v<T, __half> ? z[o][k] * by[o0 + o] : z[o][k], f[k]);
+                        for (int k = 0; k < 4; ++k) split_pieces<T, P::SETS>(std::is_same_v<T, __half> ? z[o][k] * by[o0 + o] : z[o][k], f[k]);
 #pragma unroll
                         for (int piece = 0; piece < P::PIECES; ++piece)
                             *reinterpret_cast<uint2*>(to + ((o0 + o) * P::PIECES + piece) * ap + kq) =
