@@ -175,7 +175,8 @@ class PagedKVCache:
         return CacheBatch(slots, counts, tuple(lengths), max(lengths, default=0), ids[:len(slots)], ids[len(slots):], tuple(self._stamp[s] for s in slots))
 
     def fork(self, slot: int, n: int = 1) -> List[int]:
-        """n copies of a sequence, which share its pages; returns their slots.  Only its queries are copied now."""
+        """n copies of a sequence, which share its pages; returns their slots.  Only its queries are copied now, so a batch of the sequence that
+        extend() gave before is stale: what is appended later would reach the shared pages, but not the copies' queries."""
         self._check(slot)
         if n < 0:
             raise MTALibraryError(f"fork: {n} copies")
@@ -191,6 +192,7 @@ class PagedKVCache:
             self._stamp[new] += 1
             made.append(new)
         if made:
+            self._stamp[slot] += 1
             self._upload([(s, self._len[s]) for s in made], [(s, i, p) for s in made for i, p in enumerate(self._pages[s])])
             if self._len[slot]:
                 self._copy([], [(slot, s) for s in made])
@@ -254,7 +256,7 @@ class PagedKVCache:
         return self.q_hist[layer], self.k_pages[layer], self.v_pages[layer], self.table, self.lengths
 
     def check_batch(self, batch: CacheBatch) -> None:
-        """Raises if a sequence of the batch was extended, freed or moved after extend() gave it."""
+        """Raises if a sequence of the batch was extended, forked, freed or moved after extend() gave it."""
         for s, stamp in zip(batch.slots, batch.stamps):
             if self._stamp[s] != stamp:
                 raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend()")
