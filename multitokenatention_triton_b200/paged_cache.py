@@ -75,6 +75,7 @@ class PagedKVCache:
         self._pages: List[Optional[List[int]]] = [None] * max_sequences   # of each sequence, in order; None: the slot is free
         self._len = [0] * max_sequences
         self._stamp = [0] * max_sequences                                 # changes whenever a sequence's tokens or pages do
+        self._captured: List[CacheBatch] = []                             # whose ids graphs read
 
     # ---- what is there -------------------------------------------------------------------------------------------------
 
@@ -271,12 +272,18 @@ class PagedKVCache:
 
     def append(self, batch: CacheBatch, xk: torch.Tensor, xv: torch.Tensor, xq: torch.Tensor, layer: int = 0) -> None:
         """Writes the batch's new tokens of one layer: xk, xv (B,kv heads,T,D), xq (B,H,T,D) with T >= every count; tokens behind a row's count are
-        not read."""
+        not read.  Inside a graph capture the cache keeps the batch's ids for as long as it lives itself: replays write the newest tokens of the
+        same sequences."""
         self.check_batch(batch)
         if xk.dim() != 4 or xk.shape[0] != len(batch.slots) or (batch.counts and max(batch.counts) > xk.shape[2]):
             raise MTALibraryError(f"append: keys {tuple(xk.shape)} for {len(batch.slots)} sequences with up to {max(batch.counts, default=0)} new tokens")
+        if self._capturing() and (not self._captured or self._captured[-1] is not batch):
+            self._captured.append(batch)                    # the graph's replays read its ids, which the caller need not keep
         q_hist, k_pages, v_pages, table, lengths = self.layer(layer)
         ops.cache_append(xk, xv, xq, k_pages, v_pages, q_hist, table, lengths, slots=batch.slot_ids, counts=batch.count_ids)
+
+    def _capturing(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
     def check(self) -> None:
         """Waits for the device and raises if a call over the cache met something out of range (a table or lengths written by other hands)."""

@@ -1,4 +1,7 @@
 """What becomes of tokens that PagedKVCache.extend() has reserved, on the CPU: the copies and writes that its kernels make stood in for."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -70,3 +73,23 @@ def test_a_fork_between_two_layers_of_a_prompt(plain_calls):
     c.fork(a)
     with pytest.raises(MTALibraryError, match="stale"):
         put(c, batch, [[1, 2, 3]], layers=[1])
+
+
+def test_a_captured_batch_is_kept(plain_calls, monkeypatch):
+    """A graph reads the ids of the batch that it was captured with: they live as long as the cache, whatever the caller binds anew."""
+    c = small()
+    a, b = c.add(), c.add()
+    put(c, c.extend([a, b], [3, 2]), [[1, 2, 3], [4, 5]])
+    alive = []
+    for capturing in (False, True):
+        monkeypatch.setattr(PagedKVCache, "_capturing", lambda self, on=capturing: on)
+        batch = c.extend([b, a], 1)
+        put(c, batch, [[6], [7]])
+        alive.append((weakref.ref(batch.slot_ids), weakref.ref(batch.count_ids)))
+        if capturing:
+            assert len(c._captured) == 1                    # two layers, one batch
+    monkeypatch.undo()
+    batch = c.extend([a, b], 1)                             # binds the name anew
+    gc.collect()
+    assert alive[0][0]() is None and alive[0][1]() is None
+    assert alive[1][0]().tolist() == [b, a] and alive[1][1]().tolist() == [1, 1]
