@@ -57,5 +57,5 @@ class TritonConvAttention(nn.Module):
             if group > 1:
                 K, V = K.repeat_interleave(group, dim=1), V.repeat_interleave(group, dim=1)
             return ops.conv_attn_fwd(Q, K, V, self.weight, True, softmax_scale), None
-        return ops.conv_attn_decode_fwd(*cache.layer(layer), self.weight, softmax_scale, longest,
+        return ops.conv_attn_decode_fwd(*cache._layer(layer), self.weight, softmax_scale, longest,
                                         slots=batch.slot_ids), None

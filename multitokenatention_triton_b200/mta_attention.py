@@ -193,7 +193,7 @@ class MTAAttentionTriton(nn.Module):
             if group > 1:
                 xk, xv = xk.repeat_interleave(group, dim=1), xv.repeat_interleave(group, dim=1)
             return self.forward(xq, xk, xv, None, None)
-        out = ops.mta_decode_fwd(*cache.layer(layer), self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
+        out = ops.mta_decode_fwd(*cache._layer(layer), self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
                                  self.mta_conv_after_sm_triton.effective_weight(), self.wposm_triton.weight,
                                  longest, slots=batch.slot_ids)
         return out.transpose(1, 2)

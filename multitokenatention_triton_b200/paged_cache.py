@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import heapq
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import List, Optional, Sequence, Set, Tuple, Union
 
 import torch
 
@@ -76,6 +76,12 @@ class PagedKVCache:
         self._len = [0] * max_sequences
         self._stamp = [0] * max_sequences                                 # changes whenever a sequence's tokens or pages do
         self._captured: List[CacheBatch] = []                             # whose ids graphs read
+        # What append() has written: per sequence the tokens of each layer, None where replays of a graph write them unseen, and how far
+        # its queries have been written in any layer.  `_seen`: layers whose tensors were not handed out to be written by others.
+        self._written: List[Optional[List[int]]] = [None] * max_sequences
+        self._high = [0] * max_sequences
+        self._seen = [True] * n_layers
+        self._replayed: Set[int] = set()                                  # slots that a captured append names
 
     # ---- what is there -------------------------------------------------------------------------------------------------
 
@@ -104,6 +110,8 @@ class PagedKVCache:
         slot = heapq.heappop(self._free_slots)
         self._pages[slot] = []
         self._len[slot] = 0
+        self._written[slot] = None if slot in self._replayed else [0] * self.n_layers
+        self._high[slot] = 0
         self._stamp[slot] += 1
         return slot
 
@@ -125,7 +133,7 @@ class PagedKVCache:
     def extend(self, slots: Sequence[int], counts: Union[int, Sequence[int]]) -> CacheBatch:
         """Makes room for counts[b] new tokens of sequence slots[b] (one number: the same for all) and returns the batch to append and attend with.
         A page that a fork shares is copied before it is written.  Raises CacheFullError, with nothing changed, when pages or the
-        longest length do not suffice."""
+        longest length do not suffice.  The tokens count from now on: truncate() takes back those that are not appended after all."""
         slots = tuple(int(s) for s in slots)
         counts = (int(counts),) * len(slots) if isinstance(counts, int) else tuple(int(n) for n in counts)
         if len(counts) != len(slots) or any(n < 1 for n in counts):
@@ -190,6 +198,9 @@ class PagedKVCache:
             for p in self._pages[new]:
                 self._refs[p] += 1
             self._len[new] = self._len[slot]
+            old = self._written[slot]
+            self._written[new] = None if old is None or new in self._replayed else list(old)
+            self._high[new] = self._high[slot]
             self._stamp[new] += 1
             made.append(new)
         if made:
@@ -198,6 +209,33 @@ class PagedKVCache:
             if self._len[slot]:
                 self._copy([], [(slot, s) for s in made])
         return made
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Takes back what a sequence has behind its first `length` tokens, so that others can follow them: tokens that extend() reserved and whose
+        append was refused or never came, the newest token, or all.  The cache keeps the last `history` queries, and writing a token drops
+        the oldest: further back than one written token it goes only to 0 or while no query has been dropped yet."""
+        self._check(slot)
+        if not 0 <= length <= self._len[slot]:
+            raise MTALibraryError(f"truncate: sequence {slot} has {self._len[slot]} tokens, {length} were to be left")
+        if length == self._len[slot]:
+            return
+        written = self._written[slot]
+        high = self._high[slot]
+        if written is None or not all(self._seen):
+            high = max(high, self._len[slot])              # whatever was reserved may have been written
+        if length and high > self.history and length < high - 1:
+            raise MTALibraryError(f"truncate: the queries before token {length} of sequence {slot} are gone: {high} tokens were written, the cache keeps the last "
+                                  f"{self.history}")
+        pages, keep = self._pages[slot], -(-length // self.page_size)
+        for p in pages[keep:]:
+            self._release(p)
+        del pages[keep:]
+        self._len[slot] = length
+        self._high[slot] = high if length else 0
+        if written is not None:
+            self._written[slot] = [min(n, length) for n in written]
+        self._stamp[slot] += 1
+        self._upload([(slot, length)], [])
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the pools; returns how many there are.  Batches that extend() gave before are stale."""
@@ -251,13 +289,19 @@ class PagedKVCache:
         ops.cache_copy(self.k_pages, self.v_pages, ids[:n], ids[n:2 * n], self.q_hist, ids[2 * n:2 * n + m], ids[2 * n + m:])
 
     def layer(self, layer: int) -> Tuple[torch.Tensor, ...]:
-        """(q_hist, k_pages, v_pages, table, lengths) of one layer, as ops.cache_append and the decoding calls take them."""
+        """(q_hist, k_pages, v_pages, table, lengths) of one layer, as ops.cache_append and the decoding calls take them.  Whoever takes them may
+        write them: append() no longer asks whether all earlier tokens of this layer went through it."""
+        tensors = self._layer(layer)
+        self._seen[layer] = False
+        return tensors
+
+    def _layer(self, layer: int) -> Tuple[torch.Tensor, ...]:
         if not 0 <= layer < self.n_layers:
             raise MTALibraryError(f"layer {layer} of a cache of {self.n_layers}")
         return self.q_hist[layer], self.k_pages[layer], self.v_pages[layer], self.table, self.lengths
 
     def check_batch(self, batch: CacheBatch) -> None:
-        """Raises if a sequence of the batch was extended, forked, freed or moved after extend() gave it."""
+        """Raises if a sequence of the batch was extended, forked, truncated, freed or moved after extend() gave it."""
         for s, stamp in zip(batch.slots, batch.stamps):
             if self._stamp[s] != stamp:
                 raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend()")
@@ -272,15 +316,29 @@ class PagedKVCache:
 
     def append(self, batch: CacheBatch, xk: torch.Tensor, xv: torch.Tensor, xq: torch.Tensor, layer: int = 0) -> None:
         """Writes the batch's new tokens of one layer: xk, xv (B,kv heads,T,D), xq (B,H,T,D) with T >= every count; tokens behind a row's count are
-        not read.  Inside a graph capture the cache keeps the batch's ids for as long as it lives itself: replays write the newest tokens of the
-        same sequences."""
+        not read.  Raises if tokens before them were reserved and never written, which the attention would read.  Inside a graph capture the
+        cache keeps the batch's ids for as long as it lives itself: replays write the newest tokens of the same sequences."""
         self.check_batch(batch)
         if xk.dim() != 4 or xk.shape[0] != len(batch.slots) or (batch.counts and max(batch.counts) > xk.shape[2]):
             raise MTALibraryError(f"append: keys {tuple(xk.shape)} for {len(batch.slots)} sequences with up to {max(batch.counts, default=0)} new tokens")
-        if self._capturing() and (not self._captured or self._captured[-1] is not batch):
+        q_hist, k_pages, v_pages, table, lengths = self._layer(layer)
+        if self._seen[layer]:
+            for s, n, total in zip(batch.slots, batch.counts, batch.lengths):
+                written = self._written[s]
+                if written is not None and written[layer] < total - n:
+                    raise MTALibraryError(f"append: of the {total - n} tokens that sequence {s} had before, layer {layer} was given {written[layer]}: append "
+                                          "what extend() reserved, or take it back with truncate()")
+        capturing = self._capturing()
+        if capturing and (not self._captured or self._captured[-1] is not batch):
             self._captured.append(batch)                    # the graph's replays read its ids, which the caller need not keep
-        q_hist, k_pages, v_pages, table, lengths = self.layer(layer)
         ops.cache_append(xk, xv, xq, k_pages, v_pages, q_hist, table, lengths, slots=batch.slot_ids, counts=batch.count_ids)
+        for s, total in zip(batch.slots, batch.lengths):
+            if capturing:
+                self._replayed.add(s)
+                self._written[s] = None
+            elif self._written[s] is not None:
+                self._written[s][layer] = max(self._written[s][layer], total)
+            self._high[s] = max(self._high[s], total)
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()

@@ -93,3 +93,133 @@ def test_a_captured_batch_is_kept(plain_calls, monkeypatch):
     gc.collect()
     assert alive[0][0]() is None and alive[0][1]() is None
     assert alive[1][0]().tolist() == [b, a] and alive[1][1]().tolist() == [1, 1]
+
+
+def test_tokens_that_were_never_written_are_not_passed_over(plain_calls):
+    """A refused or forgotten append leaves tokens that the attention would read: the next append raises, and truncate() takes them back."""
+    c = small()
+    a, b = c.add(), c.add()
+    c.extend([a], 5)                                        # forgotten: nothing was written at all
+    with pytest.raises(MTALibraryError, match="truncate"):
+        put(c, c.extend([a], 1), [[9]])
+    c.truncate(a, 0)
+    put(c, c.extend([a, b], [3, 20]), [[1, 2, 3], list(range(20))])
+    gone = c.extend([a, b], [2, 1])                         # refused, say
+    batch = c.extend([a, b], 1)
+    for layer in (0, 1):
+        with pytest.raises(MTALibraryError, match="truncate"):
+            put(c, batch, [[9], [9]], layers=[layer])
+    c.truncate(a, 3), c.truncate(b, 20)
+    for stale in (gone, batch):
+        with pytest.raises(MTALibraryError, match="stale"):
+            put(c, stale, [[9], [9]])
+    put(c, c.extend([a, b], [1, 2]), [[4], [20, 21]])
+    for layer in (0, 1):
+        assert read(c, a, layer) == [1, 2, 3, 4] and read(c, b, layer) == list(range(22))
+
+
+def test_a_layer_that_was_left_out(plain_calls):
+    c = small()
+    a = c.add()
+    put(c, c.extend([a], 4), [[1, 2, 3, 4]])
+    put(c, c.extend([a], 1), [[5]], layers=[0])             # refused in the second layer
+    batch = c.extend([a], 1)
+    put(c, batch, [[6]], layers=[0])
+    with pytest.raises(MTALibraryError, match="layer 1 was given 4"):
+        put(c, batch, [[6]], layers=[1])
+    with pytest.raises(MTALibraryError, match="queries"):
+        c.truncate(a, 4)                                    # layer 0 has dropped a query that token 4 looks back on
+    c.truncate(a, 0)
+    put(c, c.extend([a], 6), [[1, 2, 3, 4, 5, 6]])
+    assert read(c, a, 0) == read(c, a, 1) == [1, 2, 3, 4, 5, 6]
+
+
+def test_a_fork_of_unwritten_tokens(plain_calls):
+    c = small()
+    a = c.add()
+    put(c, c.extend([a], 20), [list(range(20))])
+    c.extend([a], 1)
+    f, = c.fork(a)
+    for s in (a, f):
+        with pytest.raises(MTALibraryError, match="truncate"):
+            put(c, c.extend([s], 1), [[9]])
+        c.truncate(s, 20)
+    put(c, c.extend([f, a], [1, 2]), [[30], [40, 41]])
+    for layer in (0, 1):
+        assert read(c, f, layer) == list(range(20)) + [30] and read(c, a, layer) == list(range(20)) + [40, 41]
+
+
+def test_truncate_gives_pages_back(plain_calls):
+    c = small()
+    a = c.add()
+    put(c, c.extend([a], 20), [list(range(20))])
+    f, = c.fork(a)
+    c.extend([a], 40)
+    assert c.free_pages == 7
+    c.truncate(a, 33)
+    assert c.free_pages == 8 and c.length(a) == 33 == int(c.lengths[a])
+    c.truncate(a, 20)
+    assert c.free_pages == 9                                # the copy of the shared page stays
+    put(c, c.extend([a], 1), [[50]])
+    assert read(c, a) == list(range(20)) + [50] and read(c, f) == list(range(20))
+    c.truncate(f, 0)
+    assert c.free_pages == 10 and int(c.lengths[f]) == 0 and read(c, a) == list(range(20)) + [50]
+    c.truncate(f, 0)
+    put(c, c.extend([f], 2), [[7, 8]])
+    assert read(c, f) == [7, 8]
+    c.free(a), c.free(f)
+    assert c.free_pages == 12 and c._refs == [0] * 12
+
+
+def test_truncate_goes_back_as_far_as_the_queries_reach(plain_calls):
+    c = small()                                             # keeps three queries
+    a = c.add()
+    put(c, c.extend([a], 3), [[1, 2, 3]])
+    c.truncate(a, 1)                                        # nothing dropped yet
+    put(c, c.extend([a], 2), [[12, 13]])
+    assert read(c, a) == [1, 12, 13]
+    put(c, c.extend([a], 2), [[14, 15]])
+    c.truncate(a, 5)                                        # nothing to do
+    c.truncate(a, 4)
+    for bad in (3, 1, 5, -1):
+        with pytest.raises(MTALibraryError, match="truncate"):
+            c.truncate(a, bad)
+    put(c, c.extend([a], 1), [[25]])
+    assert read(c, a) == [1, 12, 13, 14, 25]
+    with pytest.raises(MTALibraryError, match="no sequence"):
+        c.truncate(3, 0)
+
+
+def test_what_others_write_is_not_judged(plain_calls, monkeypatch):
+    """Replays of a captured append and writes through the tensors that layer() hands out are not seen: the appends behind them are taken, and
+    truncate() takes it that all that was reserved was written."""
+    c = small()
+    a, b = c.add(), c.add()
+    put(c, c.extend([a, b], 4), [[1, 2, 3, 4]] * 2)
+    monkeypatch.setattr(PagedKVCache, "_capturing", lambda self: True)
+    put(c, c.extend([a], 1), [[5]])
+    monkeypatch.undo()
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(ops, "cache_append", lambda *args, **kw: None)
+        for _ in range(3):
+            c.extend([a], 1)                                # replays write these
+        batch = c.extend([a], 1)
+        c.append(batch, torch.zeros(1, 2, 1, 8), torch.zeros(1, 2, 1, 8), torch.zeros(1, 2, 1, 8))
+        with pytest.raises(MTALibraryError, match="queries"):
+            c.truncate(a, 7)
+        c.truncate(a, 8)
+        with pytest.raises(MTALibraryError, match="queries"):
+            c.truncate(a, 7)
+        c.free(a)
+        assert c.add() == a                                 # the graph's replays write the slot's next sequence too
+        c.extend([a], 3)
+        x = torch.zeros(1, 2, 1, 8)
+        c.append(c.extend([a], 1), x, x, x)
+        c.extend([b], 1)
+        with pytest.raises(MTALibraryError, match="layer 0 was given 4"):
+            c.append(c.extend([b], 1), x, x, x)
+        c.layer(0)
+        batch = c.extend([b], 1)
+        c.append(batch, x, x, x)
+        with pytest.raises(MTALibraryError, match="layer 1 was given 4"):
+            c.append(batch, x, x, x, 1)
