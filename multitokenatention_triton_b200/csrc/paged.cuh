@@ -171,19 +171,9 @@ template <typename T, int DMAX> struct KeyTile {
     }
 };
 
-// 16 bytes as floats, and floats rounded to 16 bytes of T.
+// 16 bytes as floats.
 __device__ __forceinline__ void unpack16(uint4 u, float (&f)[4]) {
     f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-}
-template <typename T> __device__ __forceinline__ uint4 pack16(const float* f);
-template <> __device__ __forceinline__ uint4 pack16<float>(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-}
-template <> __device__ __forceinline__ uint4 pack16<__nv_bfloat16>(const float* f) {
-    return make_uint4(pack2<__nv_bfloat16>(f[0], f[1]), pack2<__nv_bfloat16>(f[2], f[3]), pack2<__nv_bfloat16>(f[4], f[5]), pack2<__nv_bfloat16>(f[6], f[7]));
-}
-template <> __device__ __forceinline__ uint4 pack16<__half>(const float* f) {
-    return make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]), pack2<__half>(f[4], f[5]), pack2<__half>(f[6], f[7]));
 }
 
 // 16 float32 values of one head in a warp's registers: ROWLANES lanes side by side hold a row, the warp SUBS rows at a time; the
@@ -224,6 +214,30 @@ template <int GT> struct Pieces {
     // Piece in column STRIDE * y + i of a set, i < WIDTH.
     static constexpr int WIDTH = SETS == 2 ? 2 : PIECES;
     static __device__ __forceinline__ int piece_of(int set, int i) { return set == 1 && i == 1 ? 2 : i; }
+    // Products with a first piece and with the others.  The first has the weight's sign, so that an infinite value times it is what it is times the
+    // weight; the others may be zero or of the other sign, which makes NaN of it.  So where the first product is not finite it stands alone.
+    static __device__ __forceinline__ float add(float first, float others) { return fabsf(first) < INFINITY ? first + others : first; }
+    // The sums of eight elements over a head's columns from the accumulators of lane t (acc[j][0], [1] and [2], [3]: elements j and j + 4 in
+    // two columns).  STRIDE 2: those are all, h has the eight sums.  STRIDE 4: two lanes have a head, the first and second pieces and the
+    // third and nothing, and each gets the sums of four elements, the even lane those of the first four.
+    static constexpr int SUMS = STRIDE == 4 ? 4 : 8;
+    static __device__ __forceinline__ void sum_columns(float (&h)[SUMS], const float (&acc)[4][4], int t) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float a = acc[j & 3][j / 4 * 2], b = acc[j & 3][j / 4 * 2 + 1];
+            f[j] = STRIDE == 4 && (t & 1) ? a : add(a, b);
+        }
+#pragma unroll
+        for (int e = 0; e < SUMS; ++e) {
+            if constexpr (STRIDE == 4) {
+                const float give = t & 1 ? f[e] : f[e + 4], keep = t & 1 ? f[e + 4] : f[e], got = __shfl_xor_sync(0xffffffffu, give, 1);
+                h[e] = t & 1 ? add(got, keep) : add(keep, got);
+            } else {
+                h[e] = f[e];
+            }
+        }
+    }
 };
 template <typename T, int DMAX> struct ValueTile {
     static constexpr int CHUNKS = DMAX / 64;

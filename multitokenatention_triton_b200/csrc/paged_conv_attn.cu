@@ -305,37 +305,36 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm((int)sizeof(T) * DMA
 #pragma unroll
         for (int y = 0; y < GT; ++y) sums[y] = __shfl_sync(0xffffffffu, l, y * 8 * SHARES);
         if (lane % (8 * SHARES) == 0 && !all) a.part_ml[part * GT + my_head] = make_float2(m, l);
-        // Stores EPL elements of head y from element e0 on.
+        // Stores four elements of head y from element e0 on.
         auto store = [&](int y, int e0, const float* f) {
             if (all) {
-                float r[EPL];
-#pragma unroll
-                for (int e = 0; e < EPL; ++e) r[e] = f[e] / sums[y];
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((long)b * c.H + h0 + y) * c.D + e0) = pack16<T>(r);
+                T* to = static_cast<T*>(a.out) + ((long)b * c.H + h0 + y) * c.D + e0;
+                const float r[4] = {f[0] / sums[y], f[1] / sums[y], f[2] / sums[y], f[3] / sums[y]};
+                if constexpr (HALF) *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]));
+                else *reinterpret_cast<float4*>(to) = make_float4(r[0], r[1], r[2], r[3]);
             } else {
-                float* to = a.part_o + (part * GT + y) * c.D + e0;
-#pragma unroll
-                for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                *reinterpret_cast<float4*>(a.part_o + (part * GT + y) * c.D + e0) = make_float4(f[0], f[1], f[2], f[3]);
             }
         };
         if constexpr (HALF) {
             constexpr float by = std::is_same_v<T, __half> ? 1.0f / FP16_WEIGHT : 1.0f;
 #pragma unroll
             for (int i = 0; i < V::CHUNKS; ++i) {
-                float f[8];
+                float f[P::SUMS];
+                P::sum_columns(f, o[i], t4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f[j] = (o[i][j][0] + o[i][j][1]) * by;
-                    f[j + 4] = (o[i][j][2] + o[i][j][3]) * by;
-                }
-                if constexpr (P::STRIDE == 4) {                      // a head's columns are those of two lanes
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] += __shfl_xor_sync(0xffffffffu, f[e], 1);
-                }
+                for (int e = 0; e < P::SUMS; ++e) f[e] *= by;
                 const int e0 = V::element(i, g);
 #pragma unroll
-                for (int y = 0; y < GT; ++y)
-                    if (t4 == y * P::STRIDE / 2 && e0 < c.D) store(y, e0, f);
+                for (int y = 0; y < GT; ++y) {
+                    if (t4 * 2 / P::STRIDE != y || e0 >= c.D) continue;
+                    if constexpr (P::STRIDE == 4) {
+                        store(y, e0 + (t4 & 1) * 4, f);
+                    } else {
+                        store(y, e0, f);
+                        store(y, e0 + 4, f + 4);
+                    }
+                }
             }
         } else {
 #pragma unroll

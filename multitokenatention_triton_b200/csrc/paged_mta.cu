@@ -756,31 +756,16 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
                     const float back = std::is_same_v<T, __half> && mine ? 1.0f / by[head] : 1.0f;
 #pragma unroll
                     for (int i = 0; i < CH; ++i) {
-                        float f[8];
+                        float f[P::SUMS];
+                        P::sum_columns(f, acc[i], t4);
+                        const int e0 = V::element(i, g) + (P::STRIDE == 4 ? (t4 & 1) * 4 : 0);
+                        if (!mine || V::element(i, g) >= c.D) continue;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) { f[j] = acc[i][j][0] + acc[i][j][1]; f[j + 4] = acc[i][j][2] + acc[i][j][3]; }
-                        const int e0 = V::element(i, g);
-                        if constexpr (P::STRIDE == 4) {
-                            float h[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float give = t4 & 1 ? f[e] : f[e + 4], keep = t4 & 1 ? f[e + 4] : f[e];
-                                h[e] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
-                            }
-                            if (mine && e0 < c.D) {
-                                float4* at = reinterpret_cast<float4*>(to + e0 + (t4 & 1) * 4);
-                                float4 v = *at;
-                                v.x = fmaf(h[0], back, v.x); v.y = fmaf(h[1], back, v.y); v.z = fmaf(h[2], back, v.z); v.w = fmaf(h[3], back, v.w);
-                                *at = v;
-                            }
-                        } else if (e0 < c.D) {
-#pragma unroll
-                            for (int e = 0; e < 8; e += 4) {
-                                float4* at = reinterpret_cast<float4*>(to + e0 + e);
-                                float4 v = *at;
-                                v.x = fmaf(f[e], back, v.x); v.y = fmaf(f[e + 1], back, v.y); v.z = fmaf(f[e + 2], back, v.z); v.w = fmaf(f[e + 3], back, v.w);
-                                *at = v;
-                            }
+                        for (int e = 0; e < P::SUMS; e += 4) {
+                            float4* at = reinterpret_cast<float4*>(to + e0 + e);
+                            float4 v = *at;
+                            v.x = fmaf(f[e], back, v.x); v.y = fmaf(f[e + 1], back, v.y); v.z = fmaf(f[e + 2], back, v.z); v.w = fmaf(f[e + 3], back, v.w);
+                            *at = v;
                         }
                     }
                 }

@@ -1,10 +1,10 @@
 """The product of one new token's weights with the values: how many bits the weights have, for any number of heads that share
-keys."""
+keys; values that are infinite."""
 import pytest
 import torch
 
 from multitokenatention_triton_b200 import ops
-from paged_ref import HALF_STEP, Pool
+from paged_ref import HALF_STEP, Pool, assert_near, mta_weights, token64
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -46,3 +46,29 @@ def test_weights_keep_the_bits_of_float32(mta, H, kv, dtype):
     allowed = p0[..., None] / l * c.double() * 2.0 ** -19.5 + HALF_STEP[dtype] * ref.abs()
     off = (got[:, :, 0].double() - ref).abs()
     assert bool((off <= allowed).all()), f"{int((off > allowed).sum())} of {off.numel()} off by more than allowed, the worst {float((off / allowed).max()):.1f} times"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("H,kv", [(4, 4), (4, 2), (4, 1), (8, 1)])
+@pytest.mark.parametrize("mta", [True, False])
+def test_infinite_values(mta, H, kv, dtype):
+    """An infinite value times a positive weight is that infinity, whatever numbers the weight is split into; two of both signs make NaN; every
+    other element is as if there were none.  Lengths of one run and of many."""
+    lens, D = [40, 900, 17], 64
+    pool = Pool(lens, H, kv, D, 32, 8, dtype, DEV)
+    for s, n in enumerate(lens):
+        for key, e, x in ((3, 5, 1.0), (n - 1, 6, -1.0), (n // 2, 40, 1.0), (0, 63, 1.0), (n - 2, 63, -1.0)):
+            pool.v[s][:, key, e] = x * float("inf")
+            pool.v_pages[pool.table[s, key // 32], :, key % 32, e] = x * float("inf")
+    w1, _, w2, _ = mta_weights(H, (6, 11), (3, 3), dtype, DEV)
+    eye = torch.eye(H, device=DEV, dtype=dtype)
+    w = (w1, eye, w2.abs(), eye) if mta else (w1,)
+    got = ops.mta_decode_fwd(*pool.tensors(), *w, 900) if mta else ops.conv_attn_decode_fwd(*pool.tensors(), w1, 0.125, 900)
+    wild = torch.zeros(D, dtype=torch.bool, device=DEV)
+    wild[[5, 6, 40, 63]] = True
+    for s in range(len(lens)):
+        ref, bound = token64(pool.q[s], pool.k[s], pool.v[s], w1, 0.125, *w[1:])
+        row = got[s, :, 0]
+        assert_near(row[:, ~wild], ref[:, ~wild], bound[:, ~wild], f"row {s}")
+        assert bool((row[:, 5] == float("inf")).all() and (row[:, 6] == -float("inf")).all() and (row[:, 40] == float("inf")).all()), row[:, wild]
+        assert bool(row[:, 63].isnan().all())
