@@ -53,6 +53,7 @@ class TritonConvAttention(nn.Module):
         longest = cache.longest(batch, max_length)
         cache.append(batch, K, V, Q, layer)
         if prompt:
+            Q, K, V = batch.without_padding(Q, K, V)
             group = Q.size(1) // K.size(1)
             if group > 1:
                 K, V = K.repeat_interleave(group, dim=1), V.repeat_interleave(group, dim=1)

@@ -189,6 +189,7 @@ class MTAAttentionTriton(nn.Module):
         longest = cache.longest(batch, max_length)
         cache.append(batch, xk, xv, xq, layer)
         if prompt:
+            xq, xk, xv = batch.without_padding(xq, xk, xv)
             group = xq.size(1) // xk.size(1)
             if group > 1:
                 xk, xv = xk.repeat_interleave(group, dim=1), xv.repeat_interleave(group, dim=1)

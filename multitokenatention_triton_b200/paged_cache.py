@@ -41,6 +41,15 @@ class CacheBatch:
         """Whether every sequence had no token before."""
         return self.counts == self.lengths
 
+    def without_padding(self, *tokens: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+        """(B,heads,T,D) tensors with zeros behind every row's count, the same ones where there is nothing behind.  The whole-sequence forwards
+        multiply what lies behind a row with zeros, which leaves NaN of what is not finite, and padding may be anything."""
+        T = tokens[0].shape[2]
+        if min(self.counts, default=T) >= T:
+            return tokens
+        behind = torch.arange(T, device=self.count_ids.device) >= self.count_ids[:, None]
+        return tuple(t.masked_fill(behind[:, None, :, None], 0.0) for t in tokens)
+
 
 class PagedKVCache:
     """n_layers caches with one table: k_pages, v_pages (layers, pages, kv heads, page, D), q_hist (layers, sequences, history, H, D),

@@ -223,3 +223,20 @@ def test_what_others_write_is_not_judged(plain_calls, monkeypatch):
         c.append(batch, x, x, x)
         with pytest.raises(MTALibraryError, match="layer 1 was given 4"):
             c.append(batch, x, x, x, 1)
+
+
+def test_padding_is_cleared():
+    c = small()
+    slots = [c.add() for _ in range(3)]
+    x = [torch.full((3, h, 7, 8), float("nan")) for h in (2, 1)]
+    for b, n in enumerate((3, 7, 1)):
+        for t in x:
+            t[b, :, :n] = 1.0 + b
+    batch = c.extend(slots, [3, 7, 1])
+    for given, got in zip(x, batch.without_padding(*x)):
+        assert got.shape == given.shape
+        for b, n in enumerate(batch.counts):
+            assert bool((got[b, :, :n] == 1.0 + b).all()) and bool((got[b, :, n:] == 0).all())
+        assert bool(given[0, :, 3:].isnan().all())          # the caller's are as they were
+    full = c.extend([slots[0]], 7)
+    assert full.without_padding(x[0])[0] is x[0]
