@@ -8,6 +8,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
+from .paged_cache import expand_heads
 
 
 class TritonAttention(torch.autograd.Function):
@@ -51,12 +52,14 @@ class TritonConvAttention(nn.Module):
         if prompt and not batch.from_empty:
             raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
         longest = cache.longest(batch, max_length)
-        cache.append(batch, K, V, Q, layer)
+        # as in MTAAttentionTriton.forward_cached: refusals before the first write
+        cache.check_reader("TritonConvAttention", self.channels, self.query_history)
+        ops.check_decode("conv_attn_decode", 1 if prompt else len(batch.slots), cache.n_heads, cache.n_kv_heads, cache.head_dim, *self.kernel_size, longest)
         if prompt:
-            Q, K, V = batch.without_padding(Q, K, V)
-            group = Q.size(1) // K.size(1)
-            if group > 1:
-                K, V = K.repeat_interleave(group, dim=1), V.repeat_interleave(group, dim=1)
-            return ops.conv_attn_fwd(Q, K, V, self.weight, True, softmax_scale), None
+            cache.check_step(batch, K, layer)
+            out = ops.conv_attn_fwd(*expand_heads(*batch.without_padding(Q, K, V)), self.weight, True, softmax_scale)
+            cache.append(batch, K, V, Q, layer)
+            return out, None
+        cache.append(batch, K, V, Q, layer)
         return ops.conv_attn_decode_fwd(*cache._layer(layer), self.weight, softmax_scale, longest,
                                         slots=batch.slot_ids), None

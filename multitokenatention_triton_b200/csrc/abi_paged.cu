@@ -29,9 +29,13 @@ int describe(PagedCache* c, const char* K, const void* q_hist, const void* k, co
     return MTA_OK;
 }
 
-int check_taps(const char* K, int cq, int ck, int rows, int ring) {
+int check_taps(const char* K, int cq, int ck, int rows) {
     MTA_REQUIRE(cq >= 1 && ck >= 1 && ck <= DECODE_MAX_TAPS, "%s: kernel %dx%d; 1 to %d key taps are supported", K, cq, ck, DECODE_MAX_TAPS);
-    MTA_REQUIRE(rows <= DECODE_MAX_ROWS, "%s: a token looks at %d queries; at most %d are supported", K, rows, DECODE_MAX_ROWS);
+    MTA_REQUIRE(cq <= DECODE_MAX_ROWS && rows <= DECODE_MAX_ROWS, "%s: a token looks at %d queries; at most %d are supported", K, rows, DECODE_MAX_ROWS);
+    return MTA_OK;
+}
+
+int check_ring(const char* K, int rows, int ring) {
     MTA_REQUIRE(rows <= ring, "%s: a token looks at %d queries, but the cache keeps %d", K, rows, ring);
     return MTA_OK;
 }
@@ -40,6 +44,27 @@ int check_batch(const char* K, int B, int max_length) {
     MTA_REQUIRE(B <= DECODE_MAX_BATCH, "%s: %d batch rows; at most %d are supported in one call", K, B, DECODE_MAX_BATCH);
     MTA_REQUIRE((long)B * max_length <= 1L << 34, "%s: %d rows of up to %d tokens; at most 2^34 tokens together are supported", K, B, max_length);
     return MTA_OK;
+}
+
+// What the shapes alone decide, of calls that the workspace sizes are asked for.
+int check_sizes(const char* K, int B, int H, int kv_heads, int D, int max_length) {
+    MTA_REQUIRE(B >= 0 && H >= 1 && kv_heads >= 1 && H % kv_heads == 0 && D >= 8 && max_length >= 0, "%s: bad sizes: %d rows, %d heads on %d of %d elements, %d tokens", K,
+                B, H, kv_heads, D, max_length);
+    return check_batch(K, B, max_length);
+}
+int conv_attn_size(const char* K, int B, int H, int kv_heads, int D, int cq, int ck, int max_length, size_t* bytes) {
+    if (int rc = check_sizes(K, B, H, kv_heads, D, max_length)) return rc;
+    if (int rc = check_taps(K, cq, ck, cq)) return rc;
+    *bytes = conv_attn_decode_workspace(B, H, kv_heads, D, cq, max_length);
+    return MTA_OK;
+}
+int mta_size(const char* K, int B, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2, int max_length, size_t* bytes) {
+    if (int rc = check_sizes(K, B, H, kv_heads, D, max_length)) return rc;
+    MTA_REQUIRE(H <= 128, "%s: %d heads; at most 128 are supported", K, H);
+    MTA_REQUIRE(cq2 >= 1 && cq2 <= DECODE_MAX_ROWS && cq <= DECODE_MAX_ROWS, "%s: %d and %d query taps", K, cq, cq2);
+    if (int rc = check_taps(K, cq, ck, cq + cq2 - 1)) return rc;
+    if (int rc = check_taps(K, cq2, ck2, cq + cq2 - 1)) return rc;
+    return mta_decode_workspace(B, H, kv_heads, D, cq, ck, cq2, ck2, max_length, bytes);
 }
 }  // namespace
 }  // namespace mta
@@ -101,8 +126,9 @@ int mta_cache_copy(void* k_pages, void* v_pages, const int* src, const int* dst,
 }
 
 size_t mta_conv_attn_decode_workspace_bytes(int B, int H, int kv_heads, int D, int cq, int ck, int max_length) {
-    if (B < 0 || H < 1 || kv_heads < 1 || H % kv_heads || D < 8 || cq < 1 || ck < 1 || max_length < 0) return 0;
-    return conv_attn_decode_workspace(B, H, kv_heads, D, cq, max_length);
+    set_error("%s", "");
+    size_t bytes = 0;
+    return conv_attn_size("conv_attn_decode", B, H, kv_heads, D, cq, ck, max_length, &bytes) ? 0 : bytes;
 }
 
 int mta_conv_attn_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const int* slot_ids, const void* w,
@@ -114,11 +140,11 @@ int mta_conv_attn_decode_fwd(const void* q_hist, const void* k_pages, const void
     if (int rc = describe(&c, K, q_hist, k_pages, v_pages, table, lengths, slot_ids, slots, table_width, pages, page, ring, H, kv_heads, D, max_length, B, dtype))
         return rc;
     MTA_REQUIRE(dtype_ok(w_dtype), "%s: unknown dtype code %d of the weight", K, w_dtype);
-    if (int rc = check_taps(K, cq, ck, cq, ring)) return rc;
-    if (int rc = check_batch(K, B, max_length)) return rc;
+    size_t need = 0;
+    if (int rc = conv_attn_size(K, B, H, kv_heads, D, cq, ck, max_length, &need)) return rc;
+    if (int rc = check_ring(K, cq, ring)) return rc;
     if (B == 0) return MTA_OK;
     MTA_REQUIRE(w && o && aligned16(o), "%s: null or unaligned pointer", K);
-    const size_t need = conv_attn_decode_workspace(B, H, kv_heads, D, cq, max_length);
     MTA_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "%s: workspace of %zu bytes (16-byte aligned) is smaller than the %zu needed", K,
                 workspace_bytes, need);
     if (int rc = check_device()) return rc;
@@ -126,9 +152,9 @@ int mta_conv_attn_decode_fwd(const void* q_hist, const void* k_pages, const void
 }
 
 size_t mta_decode_workspace_bytes(int B, int H, int kv_heads, int D, int cq, int ck, int cq2, int ck2, int max_length) {
-    if (B < 0 || H < 1 || kv_heads < 1 || H % kv_heads || D < 8 || cq < 1 || ck < 1 || cq2 < 1 || ck2 < 1 || max_length < 0) return 0;
+    set_error("%s", "");
     size_t bytes = 0;
-    return mta_decode_workspace(B, H, kv_heads, D, cq, ck, cq2, ck2, max_length, &bytes) ? 0 : bytes;
+    return mta_size("mta_decode", B, H, kv_heads, D, cq, ck, cq2, ck2, max_length, &bytes) ? 0 : bytes;
 }
 
 int mta_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const int* slot_ids, const void* w1,
@@ -140,15 +166,11 @@ int mta_decode_fwd(const void* q_hist, const void* k_pages, const void* v_pages,
     if (int rc = describe(&c, K, q_hist, k_pages, v_pages, table, lengths, slot_ids, slots, table_width, pages, page, ring, H, kv_heads, D, max_length, B, dtype))
         return rc;
     MTA_REQUIRE(dtype_ok(w_dtype), "%s: unknown dtype code %d of the weights", K, w_dtype);
-    MTA_REQUIRE(H <= 128, "%s: %d heads; at most 128 are supported", K, H);
-    MTA_REQUIRE(cq2 >= 1 && cq2 <= DECODE_MAX_ROWS && cq <= DECODE_MAX_ROWS, "%s: %d and %d query taps", K, cq, cq2);
-    if (int rc = check_taps(K, cq, ck, cq + cq2 - 1, ring)) return rc;
-    if (int rc = check_taps(K, cq2, ck2, cq + cq2 - 1, ring)) return rc;
-    if (int rc = check_batch(K, B, max_length)) return rc;
+    size_t need = 0;
+    if (int rc = mta_size(K, B, H, kv_heads, D, cq, ck, cq2, ck2, max_length, &need)) return rc;
+    if (int rc = check_ring(K, cq + cq2 - 1, ring)) return rc;
     if (B == 0) return MTA_OK;
     MTA_REQUIRE(w1 && W1 && w2 && W2 && o, "%s: null pointer", K);
-    size_t need = 0;
-    if (int rc = mta_decode_workspace(B, H, kv_heads, D, cq, ck, cq2, ck2, max_length, &need)) return rc;
     MTA_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "%s: workspace of %zu bytes (16-byte aligned) is smaller than the %zu needed", K,
                 workspace_bytes, need);
     if (int rc = check_device()) return rc;

@@ -22,6 +22,7 @@ from . import ops
 from .autograd_ops import CausalSoftmaxFunction, MTAFunction, PVFunction, QKScoresFunction
 from .convolution_2d import Conv2dTriton
 from .linear_head import TritonLinearHead
+from .paged_cache import expand_heads
 
 
 class MTAAttentionTriton(nn.Module):
@@ -187,16 +188,17 @@ class MTAAttentionTriton(nn.Module):
         if prompt and not batch.from_empty:
             raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
         longest = cache.longest(batch, max_length)
-        cache.append(batch, xk, xv, xq, layer)
+        # Whatever can be refused is refused before anything is written: a prompt too if its next tokens would be, even one by one.
+        w1, w2 = self.mta_conv_triton.effective_weight(), self.mta_conv_after_sm_triton.effective_weight()
+        cache.check_reader("MTAAttentionTriton", self.n_heads, self.query_history)
+        ops.check_decode("mta_decode", 1 if prompt else len(batch.slots), cache.n_heads, cache.n_kv_heads, cache.head_dim, *w1.shape[1:], *w2.shape[1:], longest)
         if prompt:
-            xq, xk, xv = batch.without_padding(xq, xk, xv)
-            group = xq.size(1) // xk.size(1)
-            if group > 1:
-                xk, xv = xk.repeat_interleave(group, dim=1), xv.repeat_interleave(group, dim=1)
-            return self.forward(xq, xk, xv, None, None)
-        out = ops.mta_decode_fwd(*cache._layer(layer), self.mta_conv_triton.effective_weight(), self.wpsm_triton.weight,
-                                 self.mta_conv_after_sm_triton.effective_weight(), self.wposm_triton.weight,
-                                 longest, slots=batch.slot_ids)
+            cache.check_step(batch, xk, layer)
+            out = self.forward(*expand_heads(*batch.without_padding(xq, xk, xv)), None, None)
+            cache.append(batch, xk, xv, xq, layer)
+            return out
+        cache.append(batch, xk, xv, xq, layer)
+        out = ops.mta_decode_fwd(*cache._layer(layer), w1, self.wpsm_triton.weight, w2, self.wposm_triton.weight, longest, slots=batch.slot_ids)
         return out.transpose(1, 2)
 
     def reset_mta_parameters(self, init_std=None):

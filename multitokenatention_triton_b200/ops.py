@@ -500,6 +500,15 @@ def _decode_buffers(what, q_hist, B, H, D, dev, out, workspace, nbytes):
     return out, workspace, workspace.numel() * workspace.element_size()
 
 
+def check_decode(what: str, *sizes: int) -> None:
+    """Raises where the sizes alone make the library refuse a decoding call: `what` is "mta_decode" or "conv_attn_decode", sizes are those of
+    mta_<what>_workspace_bytes."""
+    name = "mta_decode_workspace_bytes" if what == "mta_decode" else "mta_conv_attn_decode_workspace_bytes"
+    if _size(name, *sizes) == 0:
+        getattr(lib(), name)(*sizes)                         # the reason
+        check(1, what)
+
+
 def mta_decode_fwd(q_hist: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, w1: torch.Tensor,
                    W1: torch.Tensor, w2: torch.Tensor, W2: torch.Tensor, max_length: int, slots: Optional[torch.Tensor] = None,
                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -20,6 +20,9 @@ from . import ops
 from ._lib import MTALibraryError, cache_status
 
 
+_UNSEEN = 1 << 62
+
+
 class CacheFullError(MTALibraryError):
     """No page or no slot is left for what was asked; the cache is as it was."""
 
@@ -49,6 +52,12 @@ class CacheBatch:
             return tokens
         behind = torch.arange(T, device=self.count_ids.device) >= self.count_ids[:, None]
         return tuple(t.masked_fill(behind[:, None, :, None], 0.0) for t in tokens)
+
+
+def expand_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Keys and values of shared heads repeated for every query head, as the whole-sequence forwards take them."""
+    group = q.shape[1] // k.shape[1]
+    return (q, k, v) if group <= 1 else (q, k.repeat_interleave(group, dim=1), v.repeat_interleave(group, dim=1))
 
 
 class PagedKVCache:
@@ -85,11 +94,11 @@ class PagedKVCache:
         self._len = [0] * max_sequences
         self._stamp = [0] * max_sequences                                 # changes whenever a sequence's tokens or pages do
         self._captured: List[CacheBatch] = []                             # whose ids graphs read
-        # What append() has written: per sequence the tokens of each layer, None where replays of a graph write them unseen, and how far
-        # its queries have been written in any layer.  `_seen`: layers whose tensors were not handed out to be written by others.
-        self._written: List[Optional[List[int]]] = [None] * max_sequences
-        self._high = [0] * max_sequences
+        # What append() has written: per layer the tokens of each sequence, _UNSEEN where replays of a graph write them.  `_seen`: layers whose
+        # tensors were not handed out to be written by others.  `_high`: how far a sequence's queries went before it was truncated.
+        self._written = [[0] * max_sequences for _ in range(n_layers)]
         self._seen = [True] * n_layers
+        self._high = [0] * max_sequences
         self._replayed: Set[int] = set()                                  # slots that a captured append names
 
     # ---- what is there -------------------------------------------------------------------------------------------------
@@ -119,7 +128,8 @@ class PagedKVCache:
         slot = heapq.heappop(self._free_slots)
         self._pages[slot] = []
         self._len[slot] = 0
-        self._written[slot] = None if slot in self._replayed else [0] * self.n_layers
+        for written in self._written:
+            written[slot] = _UNSEEN if slot in self._replayed else 0
         self._high[slot] = 0
         self._stamp[slot] += 1
         return slot
@@ -207,8 +217,8 @@ class PagedKVCache:
             for p in self._pages[new]:
                 self._refs[p] += 1
             self._len[new] = self._len[slot]
-            old = self._written[slot]
-            self._written[new] = None if old is None or new in self._replayed else list(old)
+            for written in self._written:
+                written[new] = _UNSEEN if new in self._replayed else written[slot]
             self._high[new] = self._high[slot]
             self._stamp[new] += 1
             made.append(new)
@@ -228,10 +238,8 @@ class PagedKVCache:
             raise MTALibraryError(f"truncate: sequence {slot} has {self._len[slot]} tokens, {length} were to be left")
         if length == self._len[slot]:
             return
-        written = self._written[slot]
-        high = self._high[slot]
-        if written is None or not all(self._seen):
-            high = max(high, self._len[slot])              # whatever was reserved may have been written
+        # of what was not seen whatever was reserved may have been written
+        high = max(self._high[slot], max(min(written[slot], self._len[slot]) if seen else self._len[slot] for written, seen in zip(self._written, self._seen)))
         if length and high > self.history and length < high - 1:
             raise MTALibraryError(f"truncate: the queries before token {length} of sequence {slot} are gone: {high} tokens were written, the cache keeps the last "
                                   f"{self.history}")
@@ -241,8 +249,9 @@ class PagedKVCache:
         del pages[keep:]
         self._len[slot] = length
         self._high[slot] = high if length else 0
-        if written is not None:
-            self._written[slot] = [min(n, length) for n in written]
+        for written in self._written:
+            if written[slot] != _UNSEEN:
+                written[slot] = min(written[slot], length)
         self._stamp[slot] += 1
         self._upload([(slot, length)], [])
 
@@ -311,9 +320,9 @@ class PagedKVCache:
 
     def check_batch(self, batch: CacheBatch) -> None:
         """Raises if a sequence of the batch was extended, forked, truncated, freed or moved after extend() gave it."""
-        for s, stamp in zip(batch.slots, batch.stamps):
-            if self._stamp[s] != stamp:
-                raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend()")
+        if tuple(map(self._stamp.__getitem__, batch.slots)) != batch.stamps:
+            changed = [s for s, stamp in zip(batch.slots, batch.stamps) if self._stamp[s] != stamp]
+            raise MTALibraryError(f"the batch is stale: sequence {changed[0]} has changed since extend()")
 
     def longest(self, batch: CacheBatch, max_length: Optional[int]) -> int:
         """The longest length that an attention call over the batch is to serve: the batch's own, or a larger one."""
@@ -323,31 +332,43 @@ class PagedKVCache:
             raise MTALibraryError(f"max_length = {max_length}, but the batch has {batch.max_length} tokens and the cache at most {self.max_length}")
         return max_length
 
+    def check_reader(self, what: str, n_heads: int, history: int) -> None:
+        """Raises if an attention module of n_heads heads that looks back on `history` queries cannot read this cache."""
+        if n_heads != self.n_heads or history > self.history:
+            raise MTALibraryError(f"{what}: {n_heads} heads that look back on {history} queries, but the cache has {self.n_heads} heads and keeps {self.history} queries")
+
+    def check_step(self, batch: CacheBatch, xk: torch.Tensor, layer: int = 0) -> None:
+        """Raises where append() would: the batch is stale, the tokens are not the batch's, or tokens before them were never written."""
+        self.check_batch(batch)
+        if xk.dim() != 4 or xk.shape[0] != len(batch.slots) or (batch.counts and max(batch.counts) > xk.shape[2]):
+            raise MTALibraryError(f"append: keys {tuple(xk.shape)} for {len(batch.slots)} sequences with up to {max(batch.counts, default=0)} new tokens")
+        self._layer(layer)
+        if self._seen[layer]:
+            written = self._written[layer]
+            for s, n, total in zip(batch.slots, batch.counts, batch.lengths):
+                if written[s] < total - n:
+                    raise MTALibraryError(f"append: of the {total - n} tokens that sequence {s} had before, layer {layer} was given {written[s]}: append "
+                                          "what extend() reserved, or take it back with truncate()")
+
     def append(self, batch: CacheBatch, xk: torch.Tensor, xv: torch.Tensor, xq: torch.Tensor, layer: int = 0) -> None:
         """Writes the batch's new tokens of one layer: xk, xv (B,kv heads,T,D), xq (B,H,T,D) with T >= every count; tokens behind a row's count are
         not read.  Raises if tokens before them were reserved and never written, which the attention would read.  Inside a graph capture the
         cache keeps the batch's ids for as long as it lives itself: replays write the newest tokens of the same sequences."""
-        self.check_batch(batch)
-        if xk.dim() != 4 or xk.shape[0] != len(batch.slots) or (batch.counts and max(batch.counts) > xk.shape[2]):
-            raise MTALibraryError(f"append: keys {tuple(xk.shape)} for {len(batch.slots)} sequences with up to {max(batch.counts, default=0)} new tokens")
+        self.check_step(batch, xk, layer)
         q_hist, k_pages, v_pages, table, lengths = self._layer(layer)
-        if self._seen[layer]:
-            for s, n, total in zip(batch.slots, batch.counts, batch.lengths):
-                written = self._written[s]
-                if written is not None and written[layer] < total - n:
-                    raise MTALibraryError(f"append: of the {total - n} tokens that sequence {s} had before, layer {layer} was given {written[layer]}: append "
-                                          "what extend() reserved, or take it back with truncate()")
         capturing = self._capturing()
         if capturing and (not self._captured or self._captured[-1] is not batch):
             self._captured.append(batch)                    # the graph's replays read its ids, which the caller need not keep
         ops.cache_append(xk, xv, xq, k_pages, v_pages, q_hist, table, lengths, slots=batch.slot_ids, counts=batch.count_ids)
+        written = self._written[layer]
         for s, total in zip(batch.slots, batch.lengths):
-            if capturing:
-                self._replayed.add(s)
-                self._written[s] = None
-            elif self._written[s] is not None:
-                self._written[s][layer] = max(self._written[s][layer], total)
-            self._high[s] = max(self._high[s], total)
+            if written[s] < total:
+                written[s] = total
+        if capturing:
+            self._replayed.update(batch.slots)
+            for written in self._written:
+                for s in batch.slots:
+                    written[s] = _UNSEEN
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
