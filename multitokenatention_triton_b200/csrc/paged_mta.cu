@@ -44,7 +44,9 @@ struct MtaArgs {
     int w_dtype, B, cq, ck, cq2, ck2;
     float scale;           // log2(e) / sqrt(D), taken into the first conv's taps: logits are in base 2
     int workers, shift;    // tiles of 1 << shift keys; runs are cut between any 16
-    int kv_together;       // kv heads whose scores fit in shared memory at once
+    // The scores kernel's heads of keys: kv heads, or each of them `split` times, with a share of its query heads each, where one's query heads
+    // are too many; and how many of them have scores that fit in shared memory at once.
+    int score_heads, split, kv_together;
 };
 
 __host__ __device__ inline int round4(int x) { return (x + 3) / 4 * 4; }
@@ -258,11 +260,11 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     using K = KeyTile<T, DMAX>;
     extern __shared__ __align__(16) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int H = c.H, group = H / c.kv_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = score_taps(a.ck);
+    const int H = c.H, group = H / a.score_heads, tile = 1 << a.shift, R = a.cq + a.cq2 - 1, ckp = score_taps(a.ck);
     const int left = (a.ck - 1) / 2, hl = halo(left), hr = halo_right(a.ck), first_tap = lead(a.ck);
-    const bool whole = a.kv_together == c.kv_heads;              // all heads at once: what tiles share stays in the ring
+    const bool whole = a.kv_together == a.score_heads;           // all heads at once: what tiles share stays in the ring
     const ScoreRing ring(tile, a.ck, whole);
-    const ScoreSmem m = score_smem(a.B, H, group, c.kv_heads, a.kv_together, tile, a.cq, a.ck, a.cq2);
+    const ScoreSmem m = score_smem(a.B, H, group, a.score_heads, a.kv_together, tile, a.cq, a.ck, a.cq2);
     float *s_sm = reinterpret_cast<float*>(smem + m.s), *c_sm = reinterpret_cast<float*>(smem + m.c), *W_sm = reinterpret_cast<float*>(smem + m.W);
     const int s_other = whole ? 0 : (int)(m.s_one / 4);          // from one stage's ring to the next one's
     float2 *t_sm = reinterpret_cast<float2*>(smem + m.taps), *ml = reinterpret_cast<float2*>(smem + m.ml);
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             cur.first = first_of(cur.k0);
             cur.units = units_of(cur.k0);
             cur.place = (cur.first + cur.turn) % ring.keys;
-            const int nk = c.kv_heads - cur.hk0 < a.kv_together ? c.kv_heads - cur.hk0 : a.kv_together;
+            const int nk = a.score_heads - cur.hk0 < a.kv_together ? a.score_heads - cur.hk0 : a.kv_together;
             const int per_head = (cur.units + N - 1) / N, tasks = nk * per_head, t0 = warp * tasks / ROLE_WARPS;
             cur.tasks_left = (warp + 1) * tasks / ROLE_WARPS - t0;
             cur.hk = t0 / per_head;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             while (!cur.done && cur.tasks_left == 0) {
                 ++cur.stage;
                 cur.hk0 += a.kv_together;
-                if (cur.hk0 >= c.kv_heads) {
+                if (cur.hk0 >= a.score_heads) {
                     cur.hk0 = 0;
                     cur.k0 += tile;
                     if (cur.k0 >= cur.s.k1) {
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             if (cur.done) return false;
             task_unit = cur.unit;
             task_hk = cur.hk;
-            const long head = (long)(cur.hk0 + cur.hk) * head_stride;
+            const long head = (long)(a.split == 1 ? cur.hk0 + cur.hk : (cur.hk0 + cur.hk) / a.split) * head_stride;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit + i);    // -1 behind the last unit
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
     int stage = 0, stages = 0;                                   // of the whole run: what is not waited for at its end
     for (long x = begin; x < end;) {
         const Span s = span_at(c, before, lens, a.B, x, end);
-        stages += (s.k1 - s.k0 + tile - 1) / tile * ((c.kv_heads + a.kv_together - 1) / a.kv_together);
+        stages += (s.k1 - s.k0 + tile - 1) / tile * ((a.score_heads + a.kv_together - 1) / a.kv_together);
         x = (long)before[s.b] + s.k1 / KEYS;
     }
     int turn = 0;
@@ -494,10 +496,10 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
         for (int i = tid; i < a.cq2 * H * quads; i += ROLE_THREADS) ml[i] = make_float2(-INFINITY, 0.0f);
         const int limit = s.k1 < s.len ? s.k1 : s.len;           // keys from here on are another run's
         for (int k0 = s.k0; k0 < s.k1; k0 += tile) {
-            for (int hk0 = 0; hk0 < c.kv_heads; hk0 += a.kv_together, ++stage) {
+            for (int hk0 = 0; hk0 < a.score_heads; hk0 += a.kv_together, ++stage) {
                 barrier_sync(BAR_FULL + (stage & 1), THREADS);
                 // conv: (two heads, row, four keys) a thread
-                const int heads = (c.kv_heads - hk0 < a.kv_together ? c.kv_heads - hk0 : a.kv_together) * group;
+                const int heads = (a.score_heads - hk0 < a.kv_together ? a.score_heads - hk0 : a.kv_together) * group;
                 const int q0 = ((k0 - left - first_tap + turn + ring.keys) % ring.keys) >> 2;
                 const float* s_now = s_sm + (stage & 1) * s_other;
                 const float2* t_now = t_sm + hk0 * group / 2 * pair_taps(a.cq, a.ck);
@@ -974,7 +976,7 @@ template <typename T> __global__ void __launch_bounds__(128) mta_decode_join_ker
 constexpr size_t SMEM_MOST = 227 * 1024;
 
 struct Plan {
-    int shift, kv_together, gt, copies, workers;
+    int shift, split, kv_together, gt, copies, workers;
     size_t score_bytes, value_bytes;               // shared memory
     size_t ml_at, o_at, bytes;                     // workspace
     long pitch;
@@ -998,17 +1000,25 @@ int make_plan(Plan* p, int B, int H, int kv_heads, int D, int cq, int ck, int cq
         auto rounds = [&](int copies) { return (float)((H / p->gt * copies + ROLE_WARPS - 1) / ROLE_WARPS) / copies; };
         for (int copies = 2; copies <= tile / KEYS; copies *= 2)
             if (rounds(copies) < rounds(p->copies)) p->copies = copies;
-        for (p->kv_together = kv_heads; p->kv_together >= 1 && !fits; --p->kv_together) {
-            p->score_bytes = score_smem(B, H, group, kv_heads, p->kv_together, tile, cq, ck, cq2).bytes;
-            p->value_bytes = value_smem(B, H, D, tile, cq2, ck2, p->copies).bytes;
-            // a smaller tile before the heads are taken in parts (of whole pairs)
-            fits = p->score_bytes <= SMEM_MOST && p->value_bytes <= SMEM_MOST && (p->kv_together == kv_heads || (p->shift == 4 && p->kv_together * group % 2 == 0));
+        p->value_bytes = value_smem(B, H, D, tile, cq2, ck2, p->copies).bytes;
+        // A smaller tile before the heads are taken in parts (of whole pairs), parts of whole groups before parts of a group: every part reads
+        // its keys again.
+        const int splits = p->shift == 4 ? group : 1;
+        for (p->split = 1; p->split <= splits && !fits; ++p->split) {
+            if (group % p->split) continue;
+            const int heads = kv_heads * p->split, each = group / p->split;
+            for (p->kv_together = heads; p->kv_together >= (p->shift == 4 ? 1 : heads) && !fits; --p->kv_together) {
+                if (p->kv_together < heads && p->kv_together * each % 2) continue;
+                p->score_bytes = score_smem(B, H, each, heads, p->kv_together, tile, cq, ck, cq2).bytes;
+                fits = p->score_bytes <= SMEM_MOST && p->value_bytes <= SMEM_MOST;
+                if (fits) break;
+            }
             if (fits) break;
         }
         if (fits) break;
     }
     MTA_REQUIRE(fits, "mta_decode: %d heads of %d elements with kernels %dx%d and %dx%d need %zu and %zu bytes of shared memory, more than %zu", H, D, cq, ck,
-                cq2, ck2, score_smem(B, H, group, kv_heads, 1, 16, cq, ck, cq2).bytes, value_smem(B, H, D, 16, cq2, ck2, p->copies).bytes, SMEM_MOST);
+                cq2, ck2, p->score_bytes, value_smem(B, H, D, 16, cq2, ck2, p->copies).bytes, SMEM_MOST);
     p->pitch = (max_length + 63) / 64 * 64;
     const size_t parts = (size_t)p->workers + B;
     p->ml_at = ((size_t)B * cq2 * H * p->pitch * 4 + 255) / 256 * 256;
@@ -1061,7 +1071,7 @@ int mta_decode_launch(const PagedCache& cache, const void* w1, const void* W1, c
     a.part_o = reinterpret_cast<float*>(ws + p.o_at);
     a.pitch = p.pitch; a.B = B; a.cq = cq; a.ck = ck; a.cq2 = cq2; a.ck2 = ck2;
     a.scale = LOG2E / sqrtf((float)c.D);
-    a.workers = p.workers; a.shift = p.shift; a.kv_together = p.kv_together;
+    a.workers = p.workers; a.shift = p.shift; a.split = p.split; a.score_heads = c.kv_heads * p.split; a.kv_together = p.kv_together;
     if (dtype == MTA_F32) return launch<float>(c, a, p, st);
     return dtype == MTA_BF16 ? launch<__nv_bfloat16>(c, a, p, st) : launch<__half>(c, a, p, st);
 }

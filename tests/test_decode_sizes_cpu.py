@@ -100,3 +100,13 @@ def test_a_prompt_is_written_only_once_its_attention_has_run(monkeypatch):
     y = torch.zeros(1100, 4, 2, 8)
     TritonConvAttention(4, (3, 3)).forward_cached(y, y, y, many, many.extend([many.add() for _ in range(1100)], 2))
     assert len(calls) == 5
+
+
+@pytest.mark.parametrize("H,kv,kernel,kernel2,most", [(64, 1, (6, 11), (3, 3), 256), (128, 8, (6, 11), (3, 3), 128), (128, 128, (6, 11), (3, 3), 128),
+                                                      (32, 2, (11, 15), (11, 15), 256), (127, 1, (6, 11), (3, 3), 128), (48, 3, (11, 15), (3, 3), 256)])
+def test_groups_of_any_size_fit(H, kv, kernel, kernel2, most):
+    """What several heads that share keys need is what as many heads with keys of their own need."""
+    L = _lib.lib()
+    for D in (64, most):
+        for B in (1, 64):
+            assert L.mta_decode_workspace_bytes(B, H, kv, D, *kernel, *kernel2, 100) == L.mta_decode_workspace_bytes(B, H, H, D, *kernel, *kernel2, 100) > 0
