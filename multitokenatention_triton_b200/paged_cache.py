@@ -71,14 +71,20 @@ class PagedKVCache:
             raise MTALibraryError("PagedKVCache: all sizes are positive")
         if n_heads % kv:
             raise MTALibraryError(f"PagedKVCache: {n_heads} heads are no multiple of {kv} key-value heads")
-        if page_size < 16 or page_size & (page_size - 1):
-            raise MTALibraryError(f"PagedKVCache: a page of {page_size} tokens; a power of two from 16 on is wanted")
+        if not 16 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise MTALibraryError(f"PagedKVCache: a page of {page_size} tokens; a power of two from 16 to 65536 is wanted")
         if dtype not in ops._lib.DTYPE_CODE or head_dim % 8 or head_dim > (128 if dtype == torch.float32 else 256):
             raise MTALibraryError(f"PagedKVCache: head dimension {head_dim} in {dtype}; a multiple of 8 up to 256 (float32: 128) in float32, bfloat16 or "
                                   "float16 is wanted")
         self.n_heads, self.n_kv_heads, self.head_dim, self.page_size, self.history = n_heads, kv, head_dim, page_size, history
         self.num_pages, self.max_sequences, self.n_layers = num_pages, max_sequences, n_layers
         width = -(-max_length // page_size)
+        if width * page_size > 1 << 30 or n_layers > 16384:
+            raise MTALibraryError(f"PagedKVCache: {n_layers} layers of sequences of {max_length} tokens; up to 16384 layers and 2^30 tokens are supported")
+        row = head_dim * dtype.itemsize
+        if kv * page_size * row > 1 << 30 or history * n_heads * row > 1 << 30:
+            raise MTALibraryError(f"PagedKVCache: a page of {kv * page_size * row} bytes and {history * n_heads * row} bytes of queries a sequence; up to 1 GiB is "
+                                  "supported")
         self.max_length = max_length
         with torch.device(device):
             self.k_pages = torch.empty(n_layers, num_pages, kv, page_size, head_dim, dtype=dtype)
