@@ -11,6 +11,7 @@ current stream of the cache's device: calls from several streams are ordered by 
 from __future__ import annotations
 
 import heapq
+import itertools
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Set, Tuple, Union
 
@@ -21,6 +22,7 @@ from ._lib import MTALibraryError, cache_status
 
 
 _UNSEEN = 1 << 62
+_STAMPS = itertools.count(1)             # of all caches, so that a batch is known by its own cache only
 
 
 class CacheFullError(MTALibraryError):
@@ -98,7 +100,7 @@ class PagedKVCache:
         self._refs = [0] * num_pages
         self._pages: List[Optional[List[int]]] = [None] * max_sequences   # of each sequence, in order; None: the slot is free
         self._len = [0] * max_sequences
-        self._stamp = [0] * max_sequences                                 # changes whenever a sequence's tokens or pages do
+        self._stamp = [0] * max_sequences                                 # a new one whenever a sequence's tokens or pages change
         self._captured: List[CacheBatch] = []                             # whose ids graphs read
         # What append() has written: per layer the tokens of each sequence, _UNSEEN where replays of a graph write them.  `_seen`: layers whose
         # tensors were not handed out to be written by others.  `_high`: how far a sequence's queries went before it was truncated.
@@ -137,7 +139,7 @@ class PagedKVCache:
         for written in self._written:
             written[slot] = _UNSEEN if slot in self._replayed else 0
         self._high[slot] = 0
-        self._stamp[slot] += 1
+        self._stamp[slot] = next(_STAMPS)
         return slot
 
     def free(self, slot: int) -> None:
@@ -146,7 +148,7 @@ class PagedKVCache:
         for p in self._pages[slot]:
             self._release(p)
         self._pages[slot] = None
-        self._stamp[slot] += 1
+        self._stamp[slot] = next(_STAMPS)
         heapq.heappush(self._free_slots, slot)
         self._upload([(slot, 0)], [])
 
@@ -200,7 +202,7 @@ class PagedKVCache:
                 self._refs[fresh] = 1
                 entries.append((s, len(pages), fresh))
                 pages.append(fresh)
-            self._stamp[s] += 1
+            self._stamp[s] = next(_STAMPS)
             lengths.append(self._len[s])
         if copies:
             self._copy(copies, [])
@@ -226,10 +228,10 @@ class PagedKVCache:
             for written in self._written:
                 written[new] = _UNSEEN if new in self._replayed else written[slot]
             self._high[new] = self._high[slot]
-            self._stamp[new] += 1
+            self._stamp[new] = next(_STAMPS)
             made.append(new)
         if made:
-            self._stamp[slot] += 1
+            self._stamp[slot] = next(_STAMPS)
             self._upload([(s, self._len[s]) for s in made], [(s, i, p) for s in made for i, p in enumerate(self._pages[s])])
             if self._len[slot]:
                 self._copy([], [(slot, s) for s in made])
@@ -258,7 +260,7 @@ class PagedKVCache:
         for written in self._written:
             if written[slot] != _UNSEEN:
                 written[slot] = min(written[slot], length)
-        self._stamp[slot] += 1
+        self._stamp[slot] = next(_STAMPS)
         self._upload([(slot, length)], [])
 
     def compact(self) -> int:
@@ -273,7 +275,7 @@ class PagedKVCache:
                     continue
                 entries += [(s, i, moves[p]) for i, p in enumerate(pages) if p in moves]
                 self._pages[s] = [moves.get(p, p) for p in pages]
-                self._stamp[s] += 1
+                self._stamp[s] = next(_STAMPS)
             for a, b in moves.items():
                 self._refs[b], self._refs[a] = self._refs[a], 0
             self._free_pages = list(range(used, self.num_pages))
@@ -325,10 +327,10 @@ class PagedKVCache:
         return self.q_hist[layer], self.k_pages[layer], self.v_pages[layer], self.table, self.lengths
 
     def check_batch(self, batch: CacheBatch) -> None:
-        """Raises if a sequence of the batch was extended, forked, truncated, freed or moved after extend() gave it."""
-        if tuple(map(self._stamp.__getitem__, batch.slots)) != batch.stamps:
-            changed = [s for s, stamp in zip(batch.slots, batch.stamps) if self._stamp[s] != stamp]
-            raise MTALibraryError(f"the batch is stale: sequence {changed[0]} has changed since extend()")
+        """Raises if a sequence of the batch was extended, forked, truncated, freed or moved after extend() gave it, or if another cache's did."""
+        for s, stamp in zip(batch.slots, batch.stamps):
+            if s >= self.max_sequences or self._stamp[s] != stamp:
+                raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend(), or is another cache's")
 
     def longest(self, batch: CacheBatch, max_length: Optional[int]) -> int:
         """The longest length that an attention call over the batch is to serve: the batch's own, or a larger one."""

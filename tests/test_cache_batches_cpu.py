@@ -240,3 +240,21 @@ def test_padding_is_cleared():
         assert bool(given[0, :, 3:].isnan().all())          # the caller's are as they were
     full = c.extend([slots[0]], 7)
     assert full.without_padding(x[0])[0] is x[0]
+
+
+def test_a_batch_of_another_cache(plain_calls):
+    """Two caches whose sequences have gone through the same calls."""
+    c, d = small(), small()
+    for x in (c, d):
+        x.add()
+        put(x, x.extend([0], 4), [[1, 2, 3, 4]])
+    of_c, of_d = c.extend([0], 1), d.extend([0], 1)
+    with pytest.raises(MTALibraryError, match="another cache"):
+        put(d, of_c, [[5]])
+    put(d, of_d, [[5]])
+    big = small(sequences=9)
+    late = [big.add() for _ in range(9)][-1]
+    with pytest.raises(MTALibraryError, match="another cache"):
+        put(c, big.extend([late], 1), [[5]])
+    put(c, of_c, [[6]])
+    assert read(c, 0) == [1, 2, 3, 4, 6] and read(d, 0) == [1, 2, 3, 4, 5]
