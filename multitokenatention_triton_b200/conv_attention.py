@@ -53,13 +53,14 @@ class TritonConvAttention(nn.Module):
             raise NotImplementedError("several new tokens at once are a prompt: the sequences must have been empty")
         longest = cache.longest(batch, max_length)
         # as in MTAAttentionTriton.forward_cached: refusals before the first write
-        cache.check_reader("TritonConvAttention", self.channels, self.query_history)
+        cache.check_reader("TritonConvAttention", self.channels, self.kernel_size[0])
         ops.check_decode("conv_attn_decode", 1 if prompt else len(batch.slots), cache.n_heads, cache.n_kv_heads, cache.head_dim, *self.kernel_size, longest)
         if prompt:
             cache.check_step(batch, K, layer)
             out = ops.conv_attn_fwd(*expand_heads(*batch.without_padding(Q, K, V)), self.weight, True, softmax_scale)
             cache.append(batch, K, V, Q, layer)
             return out, None
-        cache.append(batch, K, V, Q, layer)
-        return ops.conv_attn_decode_fwd(*cache._layer(layer), self.weight, softmax_scale, longest,
+        tensors = cache._layer(layer)
+        cache._append(batch, K, V, Q, layer, tensors)
+        return ops.conv_attn_decode_fwd(*tensors, self.weight, softmax_scale, longest,
                                         slots=batch.slot_ids), None

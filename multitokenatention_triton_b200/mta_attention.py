@@ -190,15 +190,17 @@ class MTAAttentionTriton(nn.Module):
         longest = cache.longest(batch, max_length)
         # Whatever can be refused is refused before anything is written: a prompt too if its next tokens would be, even one by one.
         w1, w2 = self.mta_conv_triton.effective_weight(), self.mta_conv_after_sm_triton.effective_weight()
-        cache.check_reader("MTAAttentionTriton", self.n_heads, self.query_history)
-        ops.check_decode("mta_decode", 1 if prompt else len(batch.slots), cache.n_heads, cache.n_kv_heads, cache.head_dim, *w1.shape[1:], *w2.shape[1:], longest)
+        s1, s2 = w1.shape, w2.shape
+        cache.check_reader("MTAAttentionTriton", s1[0], s1[1] + s2[1] - 1)
+        ops.check_decode("mta_decode", 1 if prompt else len(batch.slots), cache.n_heads, cache.n_kv_heads, cache.head_dim, s1[1], s1[2], s2[1], s2[2], longest)
         if prompt:
             cache.check_step(batch, xk, layer)
             out = self.forward(*expand_heads(*batch.without_padding(xq, xk, xv)), None, None)
             cache.append(batch, xk, xv, xq, layer)
             return out
-        cache.append(batch, xk, xv, xq, layer)
-        out = ops.mta_decode_fwd(*cache._layer(layer), w1, self.wpsm_triton.weight, w2, self.wposm_triton.weight, longest, slots=batch.slot_ids)
+        tensors = cache._layer(layer)
+        cache._append(batch, xk, xv, xq, layer, tensors)
+        out = ops.mta_decode_fwd(*tensors, w1, self.wpsm_triton.weight, w2, self.wposm_triton.weight, longest, slots=batch.slot_ids)
         return out.transpose(1, 2)
 
     def reset_mta_parameters(self, init_std=None):

@@ -500,10 +500,12 @@ def _decode_buffers(what, q_hist, B, H, D, dev, out, workspace, nbytes):
     return out, workspace, workspace.numel() * workspace.element_size()
 
 
+_DECODE_SIZE = {"mta_decode": "mta_decode_workspace_bytes", "conv_attn_decode": "mta_conv_attn_decode_workspace_bytes"}
+
+
 def check_decode(what: str, *sizes: int) -> None:
-    """Raises where the sizes alone make the library refuse a decoding call: `what` is "mta_decode" or "conv_attn_decode", sizes are those of
-    mta_<what>_workspace_bytes."""
-    name = "mta_decode_workspace_bytes" if what == "mta_decode" else "mta_conv_attn_decode_workspace_bytes"
+    """Raises where the sizes, as the workspace's call takes them, alone make the library refuse "mta_decode" or "conv_attn_decode"."""
+    name = _DECODE_SIZE[what]
     if _size(name, *sizes) == 0:
         getattr(lib(), name)(*sizes)                         # the reason
         check(1, what)

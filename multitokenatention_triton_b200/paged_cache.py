@@ -12,8 +12,9 @@ from __future__ import annotations
 
 import heapq
 import itertools
+import operator
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Set, Tuple, Union
+from typing import Dict, List, Optional, Sequence, Set, Tuple, Union
 
 import torch
 
@@ -21,7 +22,6 @@ from . import ops
 from ._lib import MTALibraryError, cache_status
 
 
-_UNSEEN = 1 << 62
 _STAMPS = itertools.count(1)             # of all caches, so that a batch is known by its own cache only
 
 
@@ -100,11 +100,11 @@ class PagedKVCache:
         self._refs = [0] * num_pages
         self._pages: List[Optional[List[int]]] = [None] * max_sequences   # of each sequence, in order; None: the slot is free
         self._len = [0] * max_sequences
-        self._stamp = [0] * max_sequences                                 # a new one whenever a sequence's tokens or pages change
+        self._stamp = dict.fromkeys(range(max_sequences), 0)              # of each slot; a new one whenever a sequence's tokens or pages change
         self._captured: List[CacheBatch] = []                             # whose ids graphs read
-        # What append() has written: per layer the tokens of each sequence, _UNSEEN where replays of a graph write them.  `_seen`: layers whose
-        # tensors were not handed out to be written by others.  `_high`: how far a sequence's queries went before it was truncated.
-        self._written = [[0] * max_sequences for _ in range(n_layers)]
+        # What append() has written: per layer the tokens of each slot.  Not judged by it: slots that replays of a graph write (`_replayed`) and
+        # layers whose tensors were handed out (not `_seen`).  `_high`: how far a sequence's queries went before it was truncated.
+        self._written: List[Dict[int, int]] = [dict.fromkeys(range(max_sequences), 0) for _ in range(n_layers)]
         self._seen = [True] * n_layers
         self._high = [0] * max_sequences
         self._replayed: Set[int] = set()                                  # slots that a captured append names
@@ -137,7 +137,7 @@ class PagedKVCache:
         self._pages[slot] = []
         self._len[slot] = 0
         for written in self._written:
-            written[slot] = _UNSEEN if slot in self._replayed else 0
+            written[slot] = 0
         self._high[slot] = 0
         self._stamp[slot] = next(_STAMPS)
         return slot
@@ -226,7 +226,7 @@ class PagedKVCache:
                 self._refs[p] += 1
             self._len[new] = self._len[slot]
             for written in self._written:
-                written[new] = _UNSEEN if new in self._replayed else written[slot]
+                written[new] = self._len[slot] if slot in self._replayed else written[slot]
             self._high[new] = self._high[slot]
             self._stamp[new] = next(_STAMPS)
             made.append(new)
@@ -247,7 +247,8 @@ class PagedKVCache:
         if length == self._len[slot]:
             return
         # of what was not seen whatever was reserved may have been written
-        high = max(self._high[slot], max(min(written[slot], self._len[slot]) if seen else self._len[slot] for written, seen in zip(self._written, self._seen)))
+        high = max(self._high[slot], max(written[slot] if seen and slot not in self._replayed else self._len[slot]
+                                         for written, seen in zip(self._written, self._seen)))
         if length and high > self.history and length < high - 1:
             raise MTALibraryError(f"truncate: the queries before token {length} of sequence {slot} are gone: {high} tokens were written, the cache keeps the last "
                                   f"{self.history}")
@@ -258,8 +259,7 @@ class PagedKVCache:
         self._len[slot] = length
         self._high[slot] = high if length else 0
         for written in self._written:
-            if written[slot] != _UNSEEN:
-                written[slot] = min(written[slot], length)
+            written[slot] = min(written[slot], length)
         self._stamp[slot] = next(_STAMPS)
         self._upload([(slot, length)], [])
 
@@ -321,16 +321,19 @@ class PagedKVCache:
         self._seen[layer] = False
         return tensors
 
-    def _layer(self, layer: int) -> Tuple[torch.Tensor, ...]:
+    def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.n_layers:
             raise MTALibraryError(f"layer {layer} of a cache of {self.n_layers}")
+
+    def _layer(self, layer: int) -> Tuple[torch.Tensor, ...]:
+        self._check_layer(layer)
         return self.q_hist[layer], self.k_pages[layer], self.v_pages[layer], self.table, self.lengths
 
     def check_batch(self, batch: CacheBatch) -> None:
         """Raises if a sequence of the batch was extended, forked, truncated, freed or moved after extend() gave it, or if another cache's did."""
-        for s, stamp in zip(batch.slots, batch.stamps):
-            if s >= self.max_sequences or self._stamp[s] != stamp:
-                raise MTALibraryError(f"the batch is stale: sequence {s} has changed since extend(), or is another cache's")
+        if tuple(map(self._stamp.get, batch.slots)) != batch.stamps:
+            changed = [s for s, stamp in zip(batch.slots, batch.stamps) if self._stamp.get(s) != stamp]
+            raise MTALibraryError(f"the batch is stale: sequence {changed[0]} has changed since extend(), or is another cache's")
 
     def longest(self, batch: CacheBatch, max_length: Optional[int]) -> int:
         """The longest length that an attention call over the batch is to serve: the batch's own, or a larger one."""
@@ -350,11 +353,13 @@ class PagedKVCache:
         self.check_batch(batch)
         if xk.dim() != 4 or xk.shape[0] != len(batch.slots) or (batch.counts and max(batch.counts) > xk.shape[2]):
             raise MTALibraryError(f"append: keys {tuple(xk.shape)} for {len(batch.slots)} sequences with up to {max(batch.counts, default=0)} new tokens")
-        self._layer(layer)
+        self._check_layer(layer)
         if self._seen[layer]:
             written = self._written[layer]
+            if not any(map(operator.lt, map(written.get, batch.slots), map(operator.sub, batch.lengths, batch.counts))):
+                return
             for s, n, total in zip(batch.slots, batch.counts, batch.lengths):
-                if written[s] < total - n:
+                if written[s] < total - n and s not in self._replayed:
                     raise MTALibraryError(f"append: of the {total - n} tokens that sequence {s} had before, layer {layer} was given {written[s]}: append "
                                           "what extend() reserved, or take it back with truncate()")
 
@@ -362,21 +367,18 @@ class PagedKVCache:
         """Writes the batch's new tokens of one layer: xk, xv (B,kv heads,T,D), xq (B,H,T,D) with T >= every count; tokens behind a row's count are
         not read.  Raises if tokens before them were reserved and never written, which the attention would read.  Inside a graph capture the
         cache keeps the batch's ids for as long as it lives itself: replays write the newest tokens of the same sequences."""
+        self._append(batch, xk, xv, xq, layer, self._layer(layer))
+
+    def _append(self, batch: CacheBatch, xk: torch.Tensor, xv: torch.Tensor, xq: torch.Tensor, layer: int, tensors: Tuple[torch.Tensor, ...]) -> None:
         self.check_step(batch, xk, layer)
-        q_hist, k_pages, v_pages, table, lengths = self._layer(layer)
+        q_hist, k_pages, v_pages, table, lengths = tensors
         capturing = self._capturing()
         if capturing and (not self._captured or self._captured[-1] is not batch):
             self._captured.append(batch)                    # the graph's replays read its ids, which the caller need not keep
         ops.cache_append(xk, xv, xq, k_pages, v_pages, q_hist, table, lengths, slots=batch.slot_ids, counts=batch.count_ids)
-        written = self._written[layer]
-        for s, total in zip(batch.slots, batch.lengths):
-            if written[s] < total:
-                written[s] = total
+        self._written[layer].update(zip(batch.slots, batch.lengths))
         if capturing:
             self._replayed.update(batch.slots)
-            for written in self._written:
-                for s in batch.slots:
-                    written[s] = _UNSEEN
 
     def _capturing(self) -> bool:
         return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
