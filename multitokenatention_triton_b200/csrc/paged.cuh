@@ -216,7 +216,6 @@ template <int GT> struct Pieces {
     static __device__ __forceinline__ int piece_of(int set, int i) { return set == 1 && i == 1 ? 2 : i; }
     // Products with a first piece and with the others.  The first has the weight's sign, so that an infinite value times it is what it is times the
     // weight; the others may be zero or of the other sign, which makes NaN of it.  So where the first product is not finite it stands alone.
-    static __device__ __forceinline__ float add(float first, float others) { return fabsf(first) < INFINITY ? first + others : first; }
     // The sums of eight elements over a head's columns from the accumulators of lane t (acc[j][0], [1] and [2], [3]: elements j and j + 4 in
     // two columns).  STRIDE 2: those are all, h has the eight sums.  STRIDE 4: two lanes have a head, the first and second pieces and the
     // third and nothing, and each gets the sums of four elements, the even lane those of the first four.
@@ -226,13 +225,15 @@ template <int GT> struct Pieces {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float a = acc[j & 3][j / 4 * 2], b = acc[j & 3][j / 4 * 2 + 1];
-            f[j] = STRIDE == 4 && (t & 1) ? a : add(a, b);
+            f[j] = a;
+            if (fabsf(a) < INFINITY && !(STRIDE == 4 && (t & 1))) f[j] += b;
         }
 #pragma unroll
         for (int e = 0; e < SUMS; ++e) {
             if constexpr (STRIDE == 4) {
                 const float give = t & 1 ? f[e] : f[e + 4], keep = t & 1 ? f[e + 4] : f[e], got = __shfl_xor_sync(0xffffffffu, give, 1);
-                h[e] = t & 1 ? add(got, keep) : add(keep, got);
+                const float sum = keep + got;                    // NaN also where the first pieces' is infinite and the third's of no use
+                h[e] = sum == sum ? sum : t & 1 ? got : keep;
             } else {
                 h[e] = f[e];
             }

@@ -46,7 +46,7 @@ struct MtaArgs {
     int workers, shift;    // tiles of 1 << shift keys; runs are cut between any 16
     // The scores kernel's heads of keys: kv heads, or each of them `split` times, with a share of its query heads each, where one's query heads
     // are too many; and how many of them have scores that fit in shared memory at once.
-    int score_heads, split, kv_together;
+    int score_heads, per_split, kv_together;       // head h of keys is kv head h * per_split >> 16
 };
 
 __host__ __device__ inline int round4(int x) { return (x + 3) / 4 * 4; }
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_scores_kernel(PagedCach
             if (cur.done) return false;
             task_unit = cur.unit;
             task_hk = cur.hk;
-            const long head = (long)(a.split == 1 ? cur.hk0 + cur.hk : (cur.hk0 + cur.hk) / a.split) * head_stride;
+            const long head = (long)((cur.hk0 + cur.hk) * a.per_split >> 16) * head_stride;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const long base = __shfl_sync(0xffffffffu, cur.at, cur.unit + i);    // -1 behind the last unit
@@ -1071,7 +1071,10 @@ int mta_decode_launch(const PagedCache& cache, const void* w1, const void* W1, c
     a.part_o = reinterpret_cast<float*>(ws + p.o_at);
     a.pitch = p.pitch; a.B = B; a.cq = cq; a.ck = ck; a.cq2 = cq2; a.ck2 = ck2;
     a.scale = LOG2E / sqrtf((float)c.D);
-    a.workers = p.workers; a.shift = p.shift; a.split = p.split; a.score_heads = c.kv_heads * p.split; a.kv_together = p.kv_together;
+    a.workers = p.workers; a.shift = p.shift; a.score_heads = c.kv_heads * p.split; a.kv_together = p.kv_together;
+    // h / split without a division in the stream of loads: h and split are at most 128, so h * (floor(2^16 / split) + 1) exceeds
+    // h * 2^16 / split by at most h < 2^16 / split
+    a.per_split = 65536 / p.split + 1;
     if (dtype == MTA_F32) return launch<float>(c, a, p, st);
     return dtype == MTA_BF16 ? launch<__nv_bfloat16>(c, a, p, st) : launch<__half>(c, a, p, st);
 }
