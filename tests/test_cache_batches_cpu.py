@@ -1,11 +1,12 @@
 """What becomes of tokens that PagedKVCache.extend() has reserved, on the CPU: the copies and writes that its kernels make stood in for."""
 import gc
+import random
 import weakref
 
 import pytest
 import torch
 
-from multitokenatention_triton_b200 import PagedKVCache, ops
+from multitokenatention_triton_b200 import CacheFullError, PagedKVCache, ops
 from multitokenatention_triton_b200._lib import MTALibraryError
 
 
@@ -258,3 +259,80 @@ def test_a_batch_of_another_cache(plain_calls):
         put(c, big.extend([late], 1), [[5]])
     put(c, of_c, [[6]])
     assert read(c, 0) == [1, 2, 3, 4, 6] and read(d, 0) == [1, 2, 3, 4, 5]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_life_with_truncations(plain_calls, seed):
+    """Extensions that are written, forgotten or written in one layer only, truncations, forks, ends and compactions, against lists of tokens:
+    what is left is what was written, and the queries that the next token looks back on are there."""
+    r = random.Random(seed)
+    c = small(pages=24, sequences=6, longest=80)
+    held, token = {}, 0
+
+    def lived(s):
+        for layer in (0, 1):
+            n = c.length(s)
+            assert n == int(c.lengths[s]) == len(held[s])
+            for pos, t in enumerate(held[s]):
+                assert float(c.k_pages[layer, int(c.table[s, pos // 16]), 0, pos % 16, 0]) == t
+            for pos in range(max(0, n - c.history + 1), n):
+                assert float(c.q_hist[layer, s, pos % c.history, 0, 0]) == held[s][pos]
+
+    for _ in range(200):
+        op = r.choice(["add", "extend", "extend", "extend", "refused", "truncate", "truncate", "fork", "free", "compact"])
+        slots = r.sample(sorted(held), r.randint(1, len(held))) if held else []
+        s = slots[0] if slots else None
+        try:
+            if op == "add":
+                held[c.add()] = []
+            elif op in ("extend", "refused") and held:
+                counts = [r.choice([1, 1, 2, 17]) for _ in slots]
+                batch = c.extend(slots, counts)
+                new = [list(range(token + 1 + sum(counts[:i]), token + 1 + sum(counts[:i + 1]))) for i in range(len(counts))]
+                token += sum(counts)
+                if op == "extend":
+                    put(c, batch, new)
+                    for x, t in zip(slots, new):
+                        held[x] = held[x] + t
+                else:
+                    half = r.random() < 0.5
+                    if half:
+                        put(c, batch, new, layers=[0])
+                    if r.random() < 0.3:
+                        c.compact()
+                    for x, n in zip(slots, counts):
+                        with pytest.raises(MTALibraryError):
+                            put(c, c.extend([x], 1), [[0]], layers=[1])
+                        try:
+                            c.truncate(x, len(held[x]))
+                        except MTALibraryError:
+                            assert half and n > 1 and len(held[x]) > 0      # layer 0 dropped queries
+                            c.truncate(x, 0)
+                            held[x] = []
+            elif op == "truncate" and held:
+                n = r.choice([0, len(held[s]), max(0, len(held[s]) - 1), r.randint(0, len(held[s]))])
+                try:
+                    c.truncate(s, n)
+                    held[s] = held[s][:n]
+                except MTALibraryError:
+                    assert 0 < n < len(held[s]) and c._high[s] + len(held[s]) > c.history
+            elif op == "fork" and held:
+                for new in c.fork(s, r.randint(0, 2)):
+                    held[new] = list(held[s])
+            elif op == "free" and held:
+                c.free(s)
+                del held[s]
+            elif op == "compact":
+                c.compact()
+        except CacheFullError:
+            for x in held:
+                if c.length(x) != len(held[x]):             # extend() of the step that was to be refused found no page
+                    c.truncate(x, len(held[x])) if len(held[x]) in (0, c.length(x) - 1) else c.truncate(x, 0)
+                    held[x] = held[x] if c.length(x) else []
+        for x in held:
+            lived(x)
+        counts = [0] * 24
+        for pages in c._pages:
+            for p in pages or ():
+                counts[p] += 1
+        assert counts == c._refs and sorted(c._free_pages) == [p for p in range(24) if counts[p] == 0]
