@@ -257,7 +257,7 @@ int mta_host_pipeline_release(void);
  * slot_ids (B) says which slot each batch row is; NULL: row b is slot b.  H is a multiple of kv_heads: query head h reads key-value
  * head h / (H / kv_heads).  D is a multiple of 8, at most 256 (float32: 128).  All pointers to queries, keys and values and the
  * workspace are 16-byte aligned.  A slot, page, length or count that is out of range is neither read nor written: such a sequence counts
- * as empty, such a page as zeros, and mta_cache_status() reports it.
+ * as empty, such a page as zeros, and mta_cache_status() reports it.  A page has at most 65536 tokens and 1 GiB, a table row 2^30 tokens.
  *
  * mta_cache_append writes new tokens: k, v (B,kv_heads,T,D) and q (B,H,T,D), `strides` the nine strides in elements of k's, v's and
  * q's batch rows, heads and tokens (multiples of 16 bytes; elements of a row are contiguous).  Row b has counts[b] <= T tokens (NULL: T),
@@ -267,12 +267,17 @@ int mta_host_pipeline_release(void);
  * (n_slots pairs), in each of `layers` pools that lie one behind another.  No destination may be named twice or be a source.
  *
  * mta_decode_fwd is the MTA module (mta_fused_fwd) for the newest token of every row: o (B,H,D).  The last cq + cq2 - 1 <= ring
- * queries are read (at most 32); kernels have at most 33 key taps, odd or even, centred as mta_conv2d_fwd centres them; H <= 128.
+ * queries are read (at most 32); kernels have at most 33 key taps, odd or even, centred as mta_conv2d_fwd centres them; H <= 128, and what a
+ * tile of 16 keys needs has to fit in 227 KB of shared memory, whatever kv_heads is: about 4 H (cq2 (21 + 3 ck2) + H + D + 88) bytes for the
+ * values and 4 H (24 cq2 + cq (ck + 3) + H) for the scores (64 heads of 128 with 6x11 and 3x3 taps fit, with 11x15 twice they do not).
  * mta_conv_attn_decode_fwd is the conv attention (mta_conv_attn_fwd, causal) likewise; it reads the last cq queries.
  * Both: an empty sequence gets zeros; no length exceeds max_length (which sizes the workspace and the split of the work: inside a
  * captured graph pass the longest that the graph is to serve; up to 2^30, times the rows up to 2^34); at most 1024 rows.  A workspace serves one
- * call at a time.  Sums, softmax statistics, scores and weights are float32;
- * the result is rounded once, so it is nearer to exact than the whole-sequence forward, which rounds between stages.
+ * call at a time; that of mta_decode_fwd holds a row of logits for every head: B * cq2 * H * max_length * 4 bytes and little else.  The two
+ * sizes are 0 where the calls refuse the shape, and mta_last_error() says why.  Sums, softmax statistics, scores and weights are float32;
+ * the result is rounded once, so it is nearer to exact than the whole-sequence forward, which rounds between stages.  An infinite value times
+ * a weight is that infinity, or NaN where the weight is zero (in fp16: below 2^-39 of the largest).  A score that is not finite
+ * may make NaN of its own sequence's result, also where a kernel's taps end less than four keys from it; other sequences are not touched.
  */
 int mta_cache_append(const void* k, const void* v, const void* q, const long long* strides, const int* counts, void* k_pages, void* v_pages,
                      void* q_hist, const int* table, const int* lengths, const int* slot_ids, int B, int T, int slots, int table_width,

@@ -13,7 +13,7 @@
 // lanes.  Runs are equal cuts of all tiles of all sequences and heads, so lengths need not be alike; a second kernel joins the
 // runs of a head.
 //
-// Measured (a graph of calls): one sequence of 131072 tokens, 16 heads, bf16, D 128 186 us, 5.8 TB/s; 32 of 1024 to 4096 tokens, fp16,
+// Measured (a graph of calls): one sequence of 131072 tokens, 16 heads, bf16, D 128 184 us, 5.8 TB/s; 32 of 1024 to 4096 tokens, fp16,
 // D 64, 11x15 taps 102 us, 3.3 TB/s (conv and softmax chains of a warp: without the conv 79 us); 8 of 2048 to 8192 tokens, 32 heads on 8 key-value
 // heads 75 us, 2.3 TB/s (instructions: four heads' convs per key); one of 517 tokens 11 us.
 #include <type_traits>
@@ -27,7 +27,7 @@ constexpr int WARPS = 4;
 // Scores stand in pairs of query rows, (row 2i, row 2i + 1) side by side, so that one packed FMA serves two tap rows.
 constexpr int RING = 3 * KEYS, RING_PITCH = 2 * RING + 8;   // floats of a pair of rows; the pitch spreads an accumulator's rows over the banks
 constexpr int P_PITCH = KEYS + 8;                           // 16-bit weights of one column of the product with the values
-constexpr float FP16_WEIGHT = 16384.0f;                     // keeps the pieces of small weights out of fp16's subnormal numbers
+constexpr float FP16_WEIGHT = 16384.0f;                     // scales weights, at most 1, so that what fp16's smallest number leaves of a piece is 2^-39
 
 struct ConvAttnArgs {
     const void* w;

@@ -15,8 +15,8 @@
 //   join    adds the runs' outputs
 // Keys and values are read once; the logits add 4 cq2 bytes written and read, mostly in L2, to the 4 D of keys and values in 16 bits.
 //
-// Measured, bf16, D 128, taps 6x11 and 3x3 (a graph of calls): 16 sequences of 8192 tokens, 32 heads 462 us, 4.65 TB/s of keys and values
-// (scores 267, values 212, join 8 under the profiler); 8 sequences of 1024 to 4096 tokens, 16 heads 80 us; one of 301 tokens 27 us.
+// Measured, bf16, D 128, taps 6x11 and 3x3 (a graph of calls): 16 sequences of 8192 tokens, 32 heads 475 us, 4.52 TB/s of keys and values
+// (scores 273, values 219, join 7 under the profiler); 8 sequences of 1024 to 4096 tokens, 16 heads 83 us; one of 301 tokens 27 us.
 // The long batch is bound by instructions and their latency (scores, when they took 291 us: 276 with every load from L1, 213 with no convs
 // and mixes), the short ones by the chain of stages: a run of 155 keys has three.
 #include <type_traits>
@@ -251,6 +251,9 @@ struct Pages {
 template <typename T, int DMAX, int NT = 1> constexpr int TOGETHER = sizeof(T) * DMAX <= 256 && NT <= 2 ? 2 : 1;
 
 // The registers of a block are dealt anew once the roles part: 168 to a thread of the memory half, 88 to one of the other, 128 * 512 in all.
+// In 16 bits that holds a head's queries and keys (values) up to D 128 at any number of rows and D 256 up to 8.  What needs more spills: D 256
+// with 16 rows 148 bytes of stores a thread, with 32 rows (128 registers of queries, 64 of keys) 1.7 KB, its values kernels 108; float32 64 to
+// 396 in the scores kernel of heads up to 64, up to 108 above.
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
@@ -826,7 +829,8 @@ __global__ void __launch_bounds__(THREADS, 1) mta_decode_values_kernel(PagedCach
     barrier_sync(BAR_MATH, ROLE_THREADS);
     if constexpr (std::is_same_v<T, __half>) {
         // Probabilities are at most 1, so a weight of head o is at most A = sum_h |W2[o,h]| sum |w2[h]|.  Times 2^14 over the power of two
-        // below A it stays under 2^15, and its pieces are out of fp16's subnormal numbers down to 2^-28 A.
+        // below A it stays under 2^15.  Its three pieces are normal numbers of fp16, and add up to it within 2^-33 of it, only while it is above
+        // about 2^-6 A (the first alone down to 2^-28 A); below that the last of them is off by half of fp16's smallest number, 2^-39 A.
         for (int h = tid; h < H; h += ROLE_THREADS) {
             float s = 0.0f;
             for (int i = 0; i < a.cq2 * ckp; ++i) s += fabsf(t_sm[h * a.cq2 * ckp + i]);
