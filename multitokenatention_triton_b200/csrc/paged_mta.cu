@@ -16,7 +16,7 @@
 // Keys and values are read once; the logits add 4 cq2 bytes written and read, mostly in L2, to the 4 D of keys and values in 16 bits.
 //
 // Measured, bf16, D 128, taps 6x11 and 3x3 (a graph of calls): 16 sequences of 8192 tokens, 32 heads 475 us, 4.52 TB/s of keys and values
-// (scores 273, values 219, join 7 under the profiler); 8 sequences of 1024 to 4096 tokens, 16 heads 83 us; one of 301 tokens 27 us.
+// (scores 274, values 220, join 7 under the profiler); 8 sequences of 1024 to 4096 tokens, 16 heads 83 us; one of 301 tokens 27 us.
 // The long batch is bound by instructions and their latency (scores, when they took 291 us: 276 with every load from L1, 213 with no convs
 // and mixes), the short ones by the chain of stages: a run of 155 keys has three.
 #include <type_traits>
