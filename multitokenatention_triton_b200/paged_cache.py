@@ -64,7 +64,8 @@ def expand_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> Tuple[tor
 
 class PagedKVCache:
     """n_layers caches with one table: k_pages, v_pages (layers, pages, kv heads, page, D), q_hist (layers, sequences, history, H, D),
-    table (sequences, pages of the longest), lengths (sequences)."""
+    table (sequences, pages of the longest), lengths (sequences).  Tokens reach them through append(); a program that writes them itself (a saved
+    prefix, say) takes them from layer(), which says so."""
 
     def __init__(self, n_heads: int, head_dim: int, num_pages: int, max_sequences: int, max_length: int, history: int, page_size: int = 64,
                  n_kv_heads: Optional[int] = None, n_layers: int = 1, dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda"):
